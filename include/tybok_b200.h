@@ -38,6 +38,7 @@ extern "C" {
 #define TYBOK_DEV_TIMEOUT_MMA 102
 #define TYBOK_DEV_TIMEOUT_CONVERT 103
 #define TYBOK_DEV_TIMEOUT_EPILOGUE 104
+#define TYBOK_DEV_BAD_INDEX 111 /* a page, slot, position or length out of range: its element was left out */
 
 int tybok_version(void);
 /* Host pointer to a thread-local, NUL-terminated description of the last failure. */
@@ -329,6 +330,52 @@ int tybok_w8x3_qkv_rope_adarms(const void* u_planes, int u_shift, const float* s
                                const void* cos_table, const void* sin_table, void* q_out, void* k_cache, void* v_cache,
                                int B, int L, int H, int G, int D, int Lcap, int key_off, int K, int token_tile,
                                int splits, int* status_word, void* stream);
+
+/* ---- paged cache of keys and values --------------------------------------------------------
+ * A pool holds num_pages pages [P][G][page_size][D] bf16 in any order of strides with unit stride along D (k_strides /
+ * v_strides: elements between pages, heads and rows, multiples of 8; host arrays).  Key j of request b lies in page
+ * block_table[b][j / page_size] at row j % page_size; a slot is page * page_size + row.  page_size is a power of two,
+ * 16 at least.  The counterpart of the padded caches [B, G, Lcap, D] that tybok_rope_store and tybok_attention take
+ * (tybok/policies/pi05/models/gemma.py:61-125 keeps one per request).
+ *
+ * tybok_page_plan: the pages of a step, from lengths on the device.  key_lens [B]: keys that each request holds; new_lens
+ * [B]: tokens it brings; finished [B] bytes or NULL: it leaves, its pages go back first, and its row starts anew at length 0.
+ * free_pages [P] is a stack of which the first *free_count entries are free pages: pages that come back are pushed in the
+ * order of requests and pages, then every request's new pages are popped in that order.  Written: the new lengths, table,
+ * stack and count (all four in place, or to other buffers; the table is dense [B][table_width]), cu_tokens [B + 1] (exclusive
+ * sums of new_lens), pos and slots [tokens] (0 and -1 behind the last token), *missing: 0, or the pages that
+ * the stack lacks, or -1 (a negative length, a row wider than the table, more than `tokens` new tokens, a stack that
+ * overflows).  With *missing != 0 nothing is granted: the state is unchanged, cu_tokens and pos are 0, slots -1. */
+int tybok_page_plan(const int* key_lens, const int* new_lens, const void* finished, const int* block_table, const int* free_pages,
+                    const int* free_count, int* key_lens_out, int* block_table_out, int* free_pages_out, int* free_count_out,
+                    int* cu_tokens, int* pos, int* slots, int* missing, int B, int table_width, int num_pages, int tokens,
+                    int page_size, void* stream);
+
+/* Norms of queries and keys for each head, rotation, and the store, in one pass over packed projection rows
+ * src [tokens][(H + 2G) * D] (bf16, row stride ld): per head x / sqrt(mean(x^2) + eps) * norm (fp32 [D]; NULL = no norm), the
+ * first `rot` channels rotated by the angles of the row's position (cos / sin fp32 [max_pos][rot / 2]; pairs i and
+ * i + rot / 2, or 2i and 2i + 1 with `paired`), one rounding to bf16.  q goes to q_out [tokens][H * D], k and the untouched
+ * v to slots[row] of their pools; rows with a negative slot store neither.  A position outside the tables or a slot outside the
+ * pool sets the status word; such a row is not stored (and its q is 0 where the position is out).  Slots must differ. */
+int tybok_head_norm_rope_store(const void* src, int64_t ld, const int* pos, const int* slots, const float* cos_table,
+                               const float* sin_table, int max_pos, int rot, int paired, const float* norm_q, const float* norm_k,
+                               float eps, void* q_out, void* k_pages, const int64_t* k_strides, void* v_pages,
+                               const int64_t* v_strides, int tokens, int H, int G, int D, int num_pages, int page_size,
+                               int* status_word, void* stream);
+
+/* Attention of new tokens over the paged cache, single tokens and long chunks in one call.  Request b brings the queries
+ * q[cu_tokens[b] .. cu_tokens[b+1]) (bf16 rows of H * D, row stride ldq) as the last of its key_lens[b] keys: query i of n sees
+ * the keys j <= key_lens[b] - n + i (causal) or all of them; a query that sees none gives 0.  out bf16 [tokens][H * D] and /
+ * or out_planes (e5m2 [3][tokens][H * D], scaled by 2^out_shift); rows of no request are 0.  What lies in pages behind a
+ * request's last key is never read into a result.  max_tokens: the most tokens that a request brings, as far as the host
+ * knows (a choice between forms, not a limit).  Lengths and pages out of range are cut, or taken as zero keys and values, and
+ * set the status word.  B <= 2048, D 128 or 256; any sign of scale. */
+int tybok_paged_attention(const void* q, int64_t ldq, const void* k_pages, const int64_t* k_strides, const void* v_pages,
+                          const int64_t* v_strides, const int* block_table, int64_t ld_table, const int* cu_tokens,
+                          const int* key_lens, void* out, void* out_planes, int out_shift, int tokens, int B, int H, int G, int D,
+                          int num_pages, int page_size, int table_width, int max_tokens, int causal, float scale, void* workspace,
+                          size_t workspace_bytes, int* status_word, void* stream);
+size_t tybok_paged_attention_workspace_bytes(int H, int G, int D, int max_tokens);
 
 /* Enable (1) / disable (0) programmatic dependent launch for every kernel of this library
  * (process-wide; default 1).  With it, a kernel's weight prefetch overlaps the tail of the

@@ -101,6 +101,13 @@ SIGNATURES = {
         [c_void_p, c_int, c_void_p, c_int, ctypes.c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
          c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     ),
+    "tybok_page_plan": (c_int, [c_void_p] * 14 + [c_int] * 5 + [c_void_p]),
+    "tybok_head_norm_rope_store": (c_int, [c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p,
+                                           c_void_p, ctypes.c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                           c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "tybok_paged_attention": (c_int, [c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_void_p, c_void_p,
+                                      c_void_p, c_void_p] + [c_int] * 11 + [ctypes.c_float, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "tybok_paged_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "tybok_w8a16_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "tybok_w8a16_linear": (
         c_int,

@@ -114,5 +114,6 @@ class Arena {
 void bind_ops(py::module_& m);
 void bind_dit(py::module_& m);
 void bind_gemma(py::module_& m);
+void bind_paged(py::module_& m);
 
 }  // namespace tbn

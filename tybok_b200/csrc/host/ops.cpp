@@ -305,4 +305,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   tbn::bind_ops(m);
   tbn::bind_dit(m);
   tbn::bind_gemma(m);
+  tbn::bind_paged(m);
 }

@@ -12,12 +12,15 @@ directly.
 
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from . import _lib
 
 EPI_NONE, EPI_GELU, EPI_RESIDUAL = 0, 1, 2
 DEFAULT_SHIFT = 4
+DEV_BAD_INDEX = 111
 
 _L = torch.library.Library("tybok_b200", "DEF")
 _L.define("split3(Tensor x, int shift) -> Tensor")
@@ -83,6 +86,15 @@ _L.define("mlp(Tensor x, Tensor gate_up, Tensor gate_up_scale, Tensor? up, Tenso
 _L.define("ffn_tail(Tensor x, Tensor shift, Tensor scale, Tensor gate, Tensor up, Tensor up_scale, Tensor? up_bias, Tensor down, "
           "Tensor down_scale, Tensor? down_bias, float eps) -> Tensor")
 
+_L.define("page_plan(Tensor key_lens, Tensor new_lens, Tensor block_table, Tensor free_pages, Tensor free_count, int tokens, "
+          "int page_size, Tensor? finished) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)")
+_L.define("page_plan_(Tensor(a!) key_lens, Tensor new_lens, Tensor(b!) block_table, Tensor(c!) free_pages, Tensor(d!) free_count, "
+          "int tokens, int page_size, Tensor? finished) -> (Tensor, Tensor, Tensor, Tensor)")
+_L.define("head_norm_rope_store(Tensor qkv, Tensor pos, Tensor slots, Tensor cos, Tensor sin, Tensor(a!) k_pages, Tensor(b!) v_pages, "
+          "int heads, Tensor? norm_q, Tensor? norm_k, float eps, bool paired) -> Tensor")
+_L.define("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor cu_tokens, Tensor key_lens, float scale, "
+          "bool causal, int? max_tokens, bool out_bf16, bool out_planes, int out_shift) -> (Tensor, Tensor)")
+
 NORM_RMS, NORM_ADARMS, NORM_LN_MODULATE, NORM_LN_AFFINE = 0, 1, 2, 3
 EPI_GEGLU_PACKED = 4
 
@@ -105,6 +117,8 @@ def check_status(device: torch.device | None = None) -> None:
     code = int(word.item())
     if code != 0:
         word.zero_()
+        if code == DEV_BAD_INDEX:
+            raise _lib.TybokError(f"device status {code}: a page, slot, position or length out of range reached a tybok_b200 kernel")
         raise _lib.TybokError(f"device status {code}: a bounded wait inside a tybok_b200 kernel ran out")
 
 
@@ -844,6 +858,89 @@ def shift_bias_rows(w8_rows: torch.Tensor, scale_rows: torch.Tensor, shift_row: 
     them) times the norm's shift row, fp32 ``[rows]``."""
     w = w8_rows.view(torch.float8_e4m3fn).float() if w8_rows.dtype == torch.uint8 else w8_rows.float()
     return ((w @ shift_row.reshape(-1).float()) * scale_rows.reshape(-1).float()).contiguous()
+
+
+class PagePlan(NamedTuple):
+    """What ``page_plan`` gives: the state after the step, then the step's own tensors (all int32)."""
+
+    key_lens: torch.Tensor     #: [B] keys that each request holds, the new ones among them
+    block_table: torch.Tensor  #: [B, width] page of every ``page_size`` keys
+    free_pages: torch.Tensor   #: [P] stack of free pages
+    free_count: torch.Tensor   #: [1] how many of them are free
+    cu_tokens: torch.Tensor    #: [B + 1] first new token of every request, and the end
+    pos: torch.Tensor          #: [tokens] position of every new token in its request; 0 behind the last
+    slots: torch.Tensor        #: [tokens] page * page_size + row of every new token; -1 behind the last
+    missing: torch.Tensor      #: [1] 0; or the pages that were missing, or -1 for lengths out of range: nothing was granted
+
+
+def _page_plan_cuda(key_lens, new_lens, block_table, free_pages, free_count, tokens, page_size, finished):
+    return _lib.native().page_plan_op(key_lens, new_lens, block_table, free_pages, free_count, tokens, page_size, finished, False)
+
+
+def _page_plan_inplace_cuda(key_lens, new_lens, block_table, free_pages, free_count, tokens, page_size, finished):
+    return _lib.native().page_plan_op(key_lens, new_lens, block_table, free_pages, free_count, tokens, page_size, finished, True)[4:]
+
+
+def _head_norm_rope_store_cuda(*args):
+    return _lib.native().head_norm_rope_store_op(*args)
+
+
+def _paged_attention_cuda(*args):
+    return _lib.native().paged_attention_op(*args)
+
+
+_L.impl("page_plan", _page_plan_cuda, "CUDA")
+_L.impl("page_plan_", _page_plan_inplace_cuda, "CUDA")
+_L.impl("head_norm_rope_store", _head_norm_rope_store_cuda, "CUDA")
+_L.impl("paged_attention", _paged_attention_cuda, "CUDA")
+
+
+def page_plan(key_lens, new_lens, block_table, free_pages, free_count, *, tokens, page_size, finished=None) -> PagePlan:
+    """The pages of a step, planned on the GPU from the requests' lengths: requests that are ``finished`` return theirs and start
+    anew at length 0, then every request gets the pages that its ``new_lens`` tokens need.  ``tokens`` is the number of token
+    rows of the step (padding behind the last token included).  The given state is left as it is; see ``tybok_page_plan``."""
+    if type(key_lens) is _Tensor:  # as w8a16_linear
+        plan = _lib.native().page_plan(key_lens, new_lens, block_table, free_pages, free_count, tokens, page_size, finished, False)
+        if plan is not None:
+            return PagePlan(*plan)
+    return PagePlan(*torch.ops.tybok_b200.page_plan(key_lens, new_lens, block_table, free_pages, free_count, tokens, page_size, finished))
+
+
+def page_plan_(key_lens, new_lens, block_table, free_pages, free_count, *, tokens, page_size, finished=None) -> PagePlan:
+    """``page_plan`` that updates the state tensors in place (the form for a captured graph)."""
+    state = (key_lens, block_table, free_pages, free_count)
+    if type(key_lens) is _Tensor:
+        plan = _lib.native().page_plan(key_lens, new_lens, block_table, free_pages, free_count, tokens, page_size, finished, True)
+        if plan is not None:
+            return PagePlan(*state, *plan[4:])
+    return PagePlan(*state, *torch.ops.tybok_b200.page_plan_(key_lens, new_lens, block_table, free_pages, free_count, tokens, page_size,
+                                                             finished))
+
+
+def head_norm_rope_store(qkv, pos, slots, cos, sin, k_pages, v_pages, *, heads, norm_q=None, norm_k=None, eps=1e-6, paired=False):
+    """RMS norm of every query and key head, rotation by position and the store of keys and values into their pages, one pass
+    over the packed projection rows ``[tokens, (H + 2G) * D]``; returns the finished q ``[tokens, H * D]``.  ``cos`` / ``sin`` fp32
+    ``[positions, R / 2]`` turn the first ``R`` channels, in halves or (``paired``) in neighbours; see
+    ``tybok_head_norm_rope_store``."""
+    if type(qkv) is _Tensor:
+        q = _lib.native().head_norm_rope_store(qkv, pos, slots, cos, sin, k_pages, v_pages, heads, norm_q, norm_k, eps, paired)
+        if q is not None:
+            return q
+    return torch.ops.tybok_b200.head_norm_rope_store(qkv, pos, slots, cos, sin, k_pages, v_pages, heads, norm_q, norm_k, eps, paired)
+
+
+def paged_attention(q, k_pages, v_pages, block_table, cu_tokens, key_lens, *, scale, causal, max_tokens=None, out_bf16=True,
+                    out_planes=False, out_shift=DEFAULT_SHIFT):
+    """Attention of each request's new tokens over the pages it holds (its new keys are the last of them); returns
+    ``(out_bf16, out_planes)`` like ``attention``.  ``max_tokens``: the most tokens that one request brings, where the host knows
+    it (only a choice between kernels); see ``tybok_paged_attention``."""
+    if type(q) is _Tensor:
+        y = _lib.native().paged_attention(q, k_pages, v_pages, block_table, cu_tokens, key_lens, scale, causal, max_tokens, out_bf16,
+                                          out_planes, out_shift)
+        if y is not None:
+            return y
+    return torch.ops.tybok_b200.paged_attention(q, k_pages, v_pages, block_table, cu_tokens, key_lens, scale, causal, max_tokens, out_bf16,
+                                                out_planes, out_shift)
 
 
 def launch_count() -> int:
