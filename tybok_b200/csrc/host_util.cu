@@ -127,6 +127,27 @@ int tensor_map_3d(CUtensorMap* out, const void* base, CUtensorMapDataType dtype,
   return TYBOK_OK;
 }
 
+int tensor_map_4d(CUtensorMap* out, const void* base, CUtensorMapDataType dtype, const uint64_t (&dims)[4], const uint64_t (&pitch)[3],
+                  const uint32_t (&box)[4]) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(TYBOK_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || ((pitch[0] | pitch[1] | pitch[2]) & 15) || box[0] * 2 > 128 || box[1] > 256 || box[2] > 256 ||
+      box[3] > 256)
+    return fail(TYBOK_ERR_ARG, "tensor map: base/pitches must be 16-byte aligned, box <= 128 bytes x 256 x 256 x 256");
+  cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]}, strides[3] = {pitch[0], pitch[1], pitch[2]};
+  cuuint32_t b[4] = {box[0], box[1], box[2], box[3]}, estr[4] = {1, 1, 1, 1};
+  const CUresult r = fn(out, dtype, 4, const_cast<void*>(base), d, strides, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    char msg[160];
+    std::snprintf(msg, sizeof(msg), "cuTensorMapEncodeTiled (4-D) failed with CUresult %d (dims %llu x %llu x %llu x %llu)", static_cast<int>(r),
+                  static_cast<unsigned long long>(dims[0]), static_cast<unsigned long long>(dims[1]),
+                  static_cast<unsigned long long>(dims[2]), static_cast<unsigned long long>(dims[3]));
+    return fail(TYBOK_ERR_CUDA, msg);
+  }
+  return TYBOK_OK;
+}
+
 }  // namespace host
 }  // namespace tb
 

@@ -57,5 +57,9 @@ int tensor_map_3d(CUtensorMap* out, const void* base, CUtensorMapDataType dtype,
                   uint64_t dim1, uint64_t dim2, uint64_t pitch1, uint64_t pitch2, uint32_t box0, uint32_t box1,
                   uint32_t box2);
 
+// 4-D variant for 16-bit elements: dims[0] innermost, pitch[i] the byte stride of dims[i + 1].
+int tensor_map_4d(CUtensorMap* out, const void* base, CUtensorMapDataType dtype, const uint64_t (&dims)[4], const uint64_t (&pitch)[3],
+                  const uint32_t (&box)[4]);
+
 }  // namespace host
 }  // namespace tb

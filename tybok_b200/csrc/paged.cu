@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(HN_THREADS) head_norm_rope_store_kernel(const 
 #pragma unroll
   for (int i = 0; i < HN_LOADS; ++i) {
     const int h = h0 + i * PER_LOAD;
-    raw[i] = h < all ? __ldg(reinterpret_cast<const uint4*>(row + static_cast<long long>(h) * D)) : uint4{};
+    raw[i] = h < all ? *reinterpret_cast<const uint4*>(row + static_cast<long long>(h) * D) : uint4{};
   }
   const int pos = p.pos[t], slot = p.slots[t];
   const bool pos_ok = pos >= 0 && pos < p.max_pos, stored = slot >= 0 && slot < p.num_slots;
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(HN_THREADS) head_norm_rope_store_kernel(const 
   if (turned && pos_ok) {
     const long long at = static_cast<long long>(pos) * half;
     if (p.paired) {
-      const float4 c = __ldg(reinterpret_cast<const float4*>(p.cos + at + (c0 >> 1))), s = __ldg(reinterpret_cast<const float4*>(p.sin + at + (c0 >> 1)));
+      const float4 c = *reinterpret_cast<const float4*>(p.cos + at + (c0 >> 1)), s = *reinterpret_cast<const float4*>(p.sin + at + (c0 >> 1));
       const float c4[4] = {c.x, c.y, c.z, c.w}, s4[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(HN_THREADS) head_norm_rope_store_kernel(const 
       const int i0 = first ? c0 : c0 - half;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float4 c = __ldg(reinterpret_cast<const float4*>(p.cos + at + i0) + j), s = __ldg(reinterpret_cast<const float4*>(p.sin + at + i0) + j);
+        const float4 c = reinterpret_cast<const float4*>(p.cos + at + i0)[j], s = reinterpret_cast<const float4*>(p.sin + at + i0)[j];
         const float c4[4] = {c.x, c.y, c.z, c.w}, s4[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(HN_THREADS) head_norm_rope_store_kernel(const 
         const float r = rsqrtf(ss * (1.f / D) + p.eps);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const float4 a = __ldg(reinterpret_cast<const float4*>(weight + c0) + j), b = __ldg(reinterpret_cast<const float4*>(weight + c0 + away * 8) + j);
+          const float4 a = reinterpret_cast<const float4*>(weight + c0)[j], b = reinterpret_cast<const float4*>(weight + c0 + away * 8)[j];
           const float a4[4] = {a.x, a.y, a.z, a.w}, b4[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
