@@ -41,6 +41,8 @@ struct PagedAttnParams {
   float plane_scale;
   int T, B, H, G, ratio, P, W, page_shift, causal;
   int tile_rows;     // query rows (token, head of the group) of a tile, at most those of the form
+  int tile_tokens;   // tokens of a tile where it holds whole ones, else 0
+  int wide_out;      // the outputs are 32-byte aligned
   int join_blocks;   // what leaving a tile to two CTAs costs, in key blocks
   float scale_log2e;     // softmax scale * log2(e), with its sign
   float abs_scale_log2e; // its magnitude, above zero, and the bit of the scores' instruction that negates Q instead
@@ -70,16 +72,20 @@ __device__ __forceinline__ bool pa_in_range(const PagedAttnParams& p, int b) {
 // Keys that the rows before `row_end` of a request see: those of the last of them.
 __device__ __forceinline__ int pa_seen(const PagedAttnParams& p, const PaRequest& r, int row_end) {
   if (!p.causal) return r.len;
-  const int token = (row_end - 1) / p.ratio;
-  return max(0, r.len - r.n + token + 1);
+  return max(0, r.len - r.n + (row_end - 1) / p.ratio + 1);
 }
 // Key blocks of a row tile; a tile that sees no key is one block of work all the same (its output is zero).
 template <int BK>
 __device__ __forceinline__ int pa_blocks(const PagedAttnParams& p, const PaRequest& r, int tile) {
-  const int seen = pa_seen(p, r, min(r.n * p.ratio, (tile + 1) * p.tile_rows));
+  // (tiles of whole tokens need no division: a tile form's, or of one row per token)
+  const int seen = p.tile_tokens ? (p.causal ? r.len - r.n + min(r.n, (tile + 1) * p.tile_tokens) : r.len)
+                                 : pa_seen(p, r, min(r.n * p.ratio, (tile + 1) * p.tile_rows));
   return max(1, (seen + BK - 1) / BK);
 }
-__device__ __forceinline__ int pa_tiles(const PagedAttnParams& p, int n) { return (n * p.ratio + p.tile_rows - 1) / p.tile_rows; }
+__device__ __forceinline__ int pa_tiles(const PagedAttnParams& p, int n) {
+  if (n * p.ratio <= p.tile_rows) return n > 0;
+  return (n * p.ratio + p.tile_rows - 1) / p.tile_rows;
+}
 
 // ws: int4 per CTA (request, key head, tile, parts of the tile that this CTA begins and others go on with; parts = 0: none), then
 // two partial tiles per CTA: [0] ends a tile begun by another CTA, [1] begins one that others go on with.
@@ -141,112 +147,126 @@ __device__ __forceinline__ void pa_store8(const PagedAttnParams& p, long long at
   }
 }
 
-// Linear numbers of the key blocks: prefix[b] of them lie before request b.  By all threads of the CTA.
-// Returns the number of row tiles (of every key head).
-template <int BK, int NT>
-__device__ long long pa_schedule(const PagedAttnParams& p, long long* prefix) {
-  __shared__ long long warp_sum[NT / 32], warp_tiles[NT / 32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  long long carry = 0, all_tiles = 0;
-  for (int base = 0; base < p.B; base += NT) {
-    const int b = base + tid;
-    PaRequest r{0, 0, 0};
-    if (b < p.B) {
-      r = pa_request(p, b);
-      if (blockIdx.x == 0 && p.status && !pa_in_range(p, b)) atomicCAS(p.status, 0, TYBOK_DEV_BAD_INDEX);
-    }
-    const int tiles = pa_tiles(p, r.n);
-    long long cost = 0;
-    const bool many = p.causal && tiles > 4;  // their sums by the whole warp
-    if (!many) {
-      if (!p.causal) cost = static_cast<long long>(tiles) * max(1, (r.len + BK - 1) / BK);
-      else
-        for (int t = 0; t < tiles; ++t) cost += pa_blocks<BK>(p, r, t);
-    }
-    for (uint32_t left = __ballot_sync(0xffffffffu, many); left; left &= left - 1) {
-      const int src = __ffs(left) - 1;
-      const PaRequest o{0, __shfl_sync(0xffffffffu, r.n, src), __shfl_sync(0xffffffffu, r.len, src)};
-      const int ot = __shfl_sync(0xffffffffu, tiles, src);
-      long long sum = 0;
-      for (int t = lane; t < ot; t += 32) sum += pa_blocks<BK>(p, o, t);
+// The line: the key blocks of all (request, key head, row tile), numbered in that order.  Whole warps ask, each for itself:
+// request 32 k + lane at a time, and the sums of such groups stay in the lanes.
+struct PaGroup {      // 32 requests
+  PaRequest r;        // this lane's
+  int tiles;
+  uint32_t cost, sum; // blocks of one of its key heads; blocks of all of them up to this lane's request
+};
+struct PaLine {
+  uint32_t blocks, tiles;
+  uint32_t sums[PA_MAX_REQUESTS / 1024];  // blocks of group 32 i + lane
+  PaGroup last;
+};
+__device__ __forceinline__ uint32_t pa_scan(uint32_t x) {  // inclusive sums over the warp
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      if (lane == src) cost = sum;
-    }
-    cost *= p.G;
-    long long x = cost;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    const int lane_tiles = __reduce_add_sync(0xffffffffu, tiles);
-    if (lane == 31) {
-      warp_sum[warp] = x;
-      warp_tiles[warp] = lane_tiles;
-    }
-    __syncthreads();
-    long long before = carry, total = carry;
-    for (int w = 0; w < NT / 32; ++w) {
-      if (w < warp) before += warp_sum[w];
-      total += warp_sum[w];
-      all_tiles += warp_tiles[w];
-    }
-    if (b < p.B) prefix[b + 1] = before + x;
-    carry = total;
-    __syncthreads();
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if ((threadIdx.x & 31) >= o) x += y;
   }
-  if (tid == 0) prefix[0] = 0;
-  __syncthreads();
-  return all_tiles * p.G;
+  return x;
+}
+// Blocks of one key head of this lane's request.
+template <int BK>
+__device__ __forceinline__ uint32_t pa_cost(const PagedAttnParams& p, const PaRequest& r, int tiles) {
+  uint32_t cost = 0;
+  if (!p.causal) return static_cast<uint32_t>(tiles) * max(1, (r.len + BK - 1) / BK);
+  const bool many = tiles > 8;  // their sums by the whole warp
+  if (!many)
+    for (int t = 0; t < tiles; ++t) cost += pa_blocks<BK>(p, r, t);
+  for (uint32_t left = __ballot_sync(0xffffffffu, many); left; left &= left - 1) {
+    const int src = __ffs(left) - 1, lane = threadIdx.x & 31;
+    const PaRequest o{0, __shfl_sync(0xffffffffu, r.n, src), __shfl_sync(0xffffffffu, r.len, src)};
+    const int n = __shfl_sync(0xffffffffu, tiles, src);
+    uint32_t sum = 0;
+    for (int t = lane; t < n; t += 32) sum += pa_blocks<BK>(p, o, t);
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == src) cost = sum;
+  }
+  return cost;
+}
+template <int BK>
+__device__ __forceinline__ PaGroup pa_group(const PagedAttnParams& p, int k) {
+  const int b = 32 * k + (threadIdx.x & 31);
+  PaGroup g;
+  g.r = {0, 0, 0};
+  if (b < p.B) g.r = pa_request(p, b);
+  g.tiles = pa_tiles(p, g.r.n);
+  g.cost = pa_cost<BK>(p, g.r, g.tiles);
+  g.sum = pa_scan(g.cost * p.G);
+  return g;
+}
+template <int BK>
+__device__ __forceinline__ PaLine pa_line(const PagedAttnParams& p) {
+  const int lane = threadIdx.x & 31;
+  PaLine line{};
+#pragma unroll 1
+  for (int k = 0; 32 * k < p.B; ++k) {
+    line.last = pa_group<BK>(p, k);
+    const uint32_t sum = __shfl_sync(0xffffffffu, line.last.sum, 31);
+#pragma unroll
+    for (int i = 0; i < PA_MAX_REQUESTS / 1024; ++i)
+      if (k == 32 * i + lane) line.sums[i] = sum;
+    line.blocks += sum;
+    line.tiles += __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(line.last.tiles)) * p.G;
+  }
+  return line;
 }
 
-// A place in the line of key blocks: block `blk` of `nblk` of row tile `tile` of key head `g` of request `b`.
+// A place in the line: block `blk` of `nblk` of row tile `tile` of key head `g` of request `b`.
 struct PaPlace {
   int b, g, tile, blk, nblk, tiles;
   PaRequest r;
 };
-// The tile that block x lies in.  By whole warps.
+// Where block x < line.blocks lies.
 template <int BK>
-__device__ PaPlace pa_locate(const PagedAttnParams& p, const long long* prefix, long long x) {
-  PaPlace at;
-  int lo = 0, hi = p.B;  // the last b with prefix[b] <= x (requests without queries have no blocks)
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (prefix[mid] <= x) lo = mid;
-    else hi = mid;
+__device__ __forceinline__ PaPlace pa_locate(const PagedAttnParams& p, const PaLine& line, uint32_t x) {
+  const int lane = threadIdx.x & 31;
+  int k = 0;
+  PaGroup g = line.last;
+  if (p.B > 32) {
+    uint32_t before = 0;
+#pragma unroll 1
+    for (int i = 0; i < PA_MAX_REQUESTS / 1024; ++i) {
+      const uint32_t sum = pa_scan(line.sums[i]) + before, past = __ballot_sync(0xffffffffu, sum <= x);
+      k += __popc(past);
+      before = __shfl_sync(0xffffffffu, sum, 31);
+      if (past != 0xffffffffu) {
+        const int at = __popc(past);
+        x -= __shfl_sync(0xffffffffu, sum, at) - __shfl_sync(0xffffffffu, line.sums[i], at);
+        break;
+      }
+    }
+    g = pa_group<BK>(p, k);
   }
-  at.b = lo;
-  at.r = pa_request(p, lo);
-  const long long per_head = (prefix[lo + 1] - prefix[lo]) / p.G;
-  long long rest = x - prefix[lo];
-  at.g = static_cast<int>(rest / per_head);
-  rest -= at.g * per_head;
-  at.tiles = pa_tiles(p, at.r.n);
+  const int src = __popc(__ballot_sync(0xffffffffu, g.sum <= x));
+  const uint32_t per_head = __shfl_sync(0xffffffffu, g.cost, src);
+  x -= __shfl_sync(0xffffffffu, g.sum, src) - per_head * p.G;
+  PaPlace at;
+  at.b = 32 * k + src;
+  at.r = {__shfl_sync(0xffffffffu, g.r.start, src), __shfl_sync(0xffffffffu, g.r.n, src), __shfl_sync(0xffffffffu, g.r.len, src)};
+  at.tiles = __shfl_sync(0xffffffffu, g.tiles, src);
+  at.g = p.G == 1 ? 0 : static_cast<int>(x / per_head);
+  x -= at.g * per_head;
   if (!p.causal) {
     at.nblk = max(1, (at.r.len + BK - 1) / BK);
-    at.tile = static_cast<int>(rest / at.nblk);
-    at.blk = static_cast<int>(rest - static_cast<long long>(at.tile) * at.nblk);
+    at.tile = static_cast<int>(x / at.nblk);
+    at.blk = static_cast<int>(x) - at.tile * at.nblk;
     return at;
   }
-  const int lane = threadIdx.x & 31;
-  for (int t0 = 0;; t0 += 32) {  // 32 tiles at a time
-    const int n = t0 + lane < at.tiles ? pa_blocks<BK>(p, at.r, t0 + lane) : 0;
-    long long sum = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += y;
-    }
-    const uint32_t past = __ballot_sync(0xffffffffu, sum > rest);
-    if (past || t0 + 32 >= at.tiles) {
-      const int i = past ? __ffs(past) - 1 : 31;
-      at.tile = t0 + i;
+#pragma unroll 1
+  for (at.tile = 0;; at.tile += 32) {  // 32 tiles at a time
+    const uint32_t n = at.tile + lane < at.tiles ? pa_blocks<BK>(p, at.r, at.tile + lane) : 0, to = pa_scan(n);
+    const uint32_t past = __ballot_sync(0xffffffffu, to <= x);
+    if (past != 0xffffffffu) {
+      const int i = __popc(past);
+      at.tile += i;
       at.nblk = __shfl_sync(0xffffffffu, n, i);
-      at.blk = static_cast<int>(rest - (__shfl_sync(0xffffffffu, sum, i) - at.nblk));
+      at.blk = static_cast<int>(x - (__shfl_sync(0xffffffffu, to, i) - at.nblk));
       return at;
     }
-    rest -= __shfl_sync(0xffffffffu, sum, 31);
+    x -= __shfl_sync(0xffffffffu, to, 31);
   }
 }
 // The tile after this one (the caller knows that there is one).
@@ -267,54 +287,65 @@ __device__ __forceinline__ void pa_next(const PagedAttnParams& p, PaPlace& at) {
   at.nblk = pa_blocks<BK>(p, at.r, at.tile);
 }
 
-// A CTA's share [x0, x1) of the line, the same for everyone who asks: equal numbers of blocks, borders moved to the edge of a tile
-// that lies near.  With `whole` every border moves to the nearest edge, so no tile has two CTAs: where the rounds of whole tiles
-// take no longer than an even share and the joining of its parts.
+// A CTA's share [x0, x1) of the line: equal numbers of blocks, borders moved to the edge of a tile that lies near.  With `whole` every
+// border moves to the nearest edge, so no tile has two CTAs: where the rounds of whole tiles take no longer than an even
+// share and the joining of its parts.
 struct PaShare {
-  long long per, x0, x1;
+  uint32_t per, x0, x1;
   bool whole;
 };
 __device__ __forceinline__ int pa_snap(const PaShare& sh, int blk, int nblk, int join_blocks) {
   const bool up = 2 * blk > nblk;
   const int away = up ? nblk - blk : blk;
-  return sh.whole || away * 4ll <= min(sh.per, 4ll * join_blocks) - 4 ? (up ? nblk : 0) : blk;
+  return sh.whole || 4 * away <= static_cast<int>(min(sh.per, 4u * join_blocks)) - 4 ? (up ? nblk : 0) : blk;
 }
 template <int BK>
-__device__ PaShare pa_share(const PagedAttnParams& p, const long long* prefix, long long tiles, PaPlace& first) {
+__device__ PaShare pa_share(const PagedAttnParams& p, PaPlace& first) {
+  const PaLine line = pa_line<BK>(p);
   PaShare sh;
-  const long long total = prefix[p.B], ctas = gridDim.x;
-  sh.per = (total + ctas - 1) / ctas;
-  sh.whole = (tiles + ctas - 1) / ctas * total <= (sh.per + p.join_blocks) * tiles;  // rounds * average length
-  auto border = [&](long long c, PaPlace& at) {
-    const long long x = c * sh.per;
-    if (x >= total) return total;
-    at = pa_locate<BK>(p, prefix, x);
-    const int blk = pa_snap(sh, at.blk, at.nblk, p.join_blocks);
-    const long long y = x - at.blk + blk;
-    at.blk = blk;
-    return y;
-  };
+  const uint32_t ctas = gridDim.x;
+  sh.per = (line.blocks + ctas - 1) / ctas;
+  // rounds * average length of a tile against an even share
+  sh.whole = static_cast<float>((line.tiles + ctas - 1) / ctas) * line.blocks <= static_cast<float>(sh.per + p.join_blocks) * line.tiles;
   PaPlace next{};
-  sh.x0 = border(blockIdx.x, first);
-  sh.x1 = border(blockIdx.x + 1ll, next);
-  if (sh.x0 < sh.x1 && first.blk == first.nblk) pa_next<BK>(p, first);
+  uint32_t border[2];
+#pragma unroll 1
+  for (int i = 1; i >= 0; --i) {
+    const unsigned long long x = static_cast<unsigned long long>(blockIdx.x + i) * sh.per;
+    border[i] = line.blocks;
+    if (x >= line.blocks) continue;
+    next = pa_locate<BK>(p, line, static_cast<uint32_t>(x));
+    const int blk = pa_snap(sh, next.blk, next.nblk, p.join_blocks);
+    border[i] = static_cast<uint32_t>(x) - next.blk + blk;
+    next.blk = blk;
+  }
+  sh.x0 = border[0];
+  sh.x1 = border[1];
+  if (sh.x0 < sh.x1 && next.blk == next.nblk) pa_next<BK>(p, next);
+  first = next;
   return sh;
 }
 // How many CTAs the tile has that begins at x in this CTA's share and goes on behind it.
-__device__ __forceinline__ int pa_parts(const PagedAttnParams& p, const PaShare& sh, long long x, int nblk) {
-  const long long last = (x + nblk - 1) / sh.per;
+__device__ __forceinline__ int pa_parts(const PagedAttnParams& p, const PaShare& sh, uint32_t x, int nblk) {
+  const uint32_t last = (x + nblk - 1) / sh.per;
   const int blk = static_cast<int>(last * sh.per - x);
-  const bool gone = last > static_cast<long long>(blockIdx.x) && blk > 0 && pa_snap(sh, blk, nblk, p.join_blocks) == nblk;  // its border moved behind the tile
+  const bool gone = last > blockIdx.x && blk > 0 && pa_snap(sh, blk, nblk, p.join_blocks) == nblk;  // its border moved behind the tile
   return static_cast<int>(last - blockIdx.x) + (gone ? 0 : 1);
+}
+// Lengths that reach beyond what they index: the status word says so (the kernels cut them).
+__device__ __forceinline__ void pa_check(const PagedAttnParams& p, int t, int nt) {
+  if (blockIdx.x != 0 || !p.status) return;
+  for (int b = t; b < p.B; b += nt)
+    if (!pa_in_range(p, b)) atomicCAS(p.status, 0, TYBOK_DEV_BAD_INDEX);
 }
 
 // Output rows that belong to no request are zero.
 template <int D>
-__device__ __forceinline__ void pa_zero_rows(const PagedAttnParams& p, int nt) {
+__device__ __forceinline__ void pa_zero_rows(const PagedAttnParams& p, int t, int nt) {
   const int first = max(0, min(p.cu[0], p.T)), last = max(first, min(p.cu[p.B], p.T));
   const long long per = p.ld_out / 8, rows = p.T - last + first, n = rows * per;
   const float zero[8] = {};
-  for (long long i = static_cast<long long>(blockIdx.x) * nt + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * nt) {
+  for (long long i = static_cast<long long>(blockIdx.x) * nt + t; i < n; i += static_cast<long long>(gridDim.x) * nt) {
     const long long row = i / per, c = i - row * per;
     pa_store8(p, (row < first ? row : row - first + last) * p.ld_out + c * 8, zero);
   }
@@ -326,21 +357,20 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_rows_kernel(const PagedAt
   __shared__ float s_m[PR_WARPS][PR_ROWS], s_l[PR_WARPS][PR_ROWS];
   constexpr int SUB = pr_sub(D), BK = pr_block(D), ROW_BYTES = D * 2, CHUNKS = D / 8, KS = D / 16;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  long long* prefix = reinterpret_cast<long long*>(pr_smem + PR_SMEM);
   if (p.pdl) {
     pdl_launch_dependents();
     pdl_wait();
   }
-  pa_zero_rows<D>(p, PR_THREADS);
-  const long long tiles = pa_schedule<BK, PR_THREADS>(p, prefix);
+  pa_check(p, tid, PR_THREADS);
+  pa_zero_rows<D>(p, tid, PR_THREADS);
   PaPlace at{};
-  const PaShare share = pa_share<BK>(p, prefix, tiles, at);
-  const long long x1 = share.x1;
-  long long x = share.x0;
+  const PaShare share = pa_share<BK>(p, at);
+  const uint32_t x1 = share.x1;
+  uint32_t x = share.x0;
   int4 header = make_int4(0, 0, 0, 0);
   const uint32_t ring = smem_u32(pr_smem) + warp * (PR_STAGES * PR_STAGE_BYTES);
   while (x < x1) {
-    const int end = static_cast<int>(min(static_cast<long long>(at.nblk), at.blk + (x1 - x)));
+    const int end = static_cast<int>(min(static_cast<uint32_t>(at.nblk), at.blk + (x1 - x)));
     const int rows = at.r.n * p.ratio;
     // this thread's two rows of the tile: queries as operand fragments, keys they see
     uint32_t qf[KS][4];
@@ -538,35 +568,33 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_rows_kernel(const PagedAt
 }
 
 // ------------------------------------------------------------------------------------------------ tile forms
-// Many rows per key head: 128-row tiles on the fifth-generation tensor cores.  Four control warps (keys, values, queries by TMA,
-// one that issues the products) and two groups of four softmax warps with one query row per thread and tensor-memory lane.  The
-// warp that fetches the queries walks the CTA's share and tells the others, a few tiles ahead; rings and barriers run on from
-// tile to tile, so the next tile's queries, keys and first scores are on their way while this one's output is written.
-//   scores   S = Q K^T into tensor memory, P = 2^(S c - m) in bf16 over it (m: a reference that moves only when a block's
-//            maximum exceeds it by more than 2^8, then the row of O is rescaled), O += P V with P read from tensor memory.
-//   head_dim 128 (paged_pair_kernel): two tiles of 128 rows share every key block of 128, a group each; the tiles take turns, one's
-//            products run under the other's exponentials.
-//   head_dim 256 (paged_wide_kernel): O of one tile takes half of the tensor memory; key blocks of 64 go round four score buffers and
-//            the groups take every other block, so that a block's softmax has the time of two blocks' products.
+// Many rows per key head: 128-row tiles on the fifth-generation tensor cores.  Four control warps (the CTA's share, keys and values,
+// one or two that issue the products) and two groups of four softmax warps with one query row per thread and tensor-memory
+// lane.  The warp that walks the CTA's share tells the others, a few tiles ahead; rings and barriers run on from tile to tile, so
+// the next tile's queries, keys and first scores are on their way while this one's output is written.
+//   S = Q K^T into tensor memory, P = 2^(S c - m) in bf16 over it (m: a reference that moves only when a block's maximum exceeds
+//   it by more than 2^8, then the row of O is rescaled), O += P V with P read from tensor memory.
+//   head_dim 128 (paged_pair_kernel): two tiles of 128 rows share every block of 128 keys, a group of softmax warps and a warp that
+//            issues products each (issuing costs 20 to 50 clocks an instruction and about 100 a wait: one warp for both tiles
+//            set the pace); queries in shared memory.  Tensor memory: S / P and O of both tiles, 128 columns each; a tile's
+//            S(j+1) follows its PV(j).  The tiles take turns: one's products run under the other's exponentials.
+//   head_dim 256 (paged_wide_kernel): O of one tile takes half of the tensor memory.  The groups take every other block of 64 keys, with a
+//            score buffer each: PV(j), S(j+2).  The queries are in tensor memory too: as a shared-memory operand their 64 KB
+//            would be read again for every 64 keys, and with the keys, the values and what the copies write, shared
+//            memory (128 bytes a clock) would set the pace (1790 clk a block).
 // A page is one box of the tensor map and 64 channels (or a block's rows of a larger page); lanes of the copying warp issue one
 // box each.  Page numbers out of range read as zero through the map's bounds.
 // Values behind a request's last key are zeroed in shared memory before their product (their weights are zero, but what lies
 // there may be anything).
 constexpr int PT_THREADS = 384;
 constexpr int PT_REGS_CONTROL = 72, PT_REGS_SOFTMAX = 216;  // launched with 168 each: 72 + 2 * 216 = 3 * 168
-constexpr int PT_SMEM = 65536 + 4 * 32768 + 1024;           // queries, two key and two value blocks
+constexpr int PT_SMEM = 196608 + 1024;  // queries, two key and two value blocks
 constexpr float PT_RESCALE = 8.0f;
 #define PA_MASKED 0xff800000u  // -infinity
 
-__host__ __device__ constexpr int pt_bk(int d) { return d == 128 ? 128 : 64; }
 __host__ __device__ constexpr int pt_rows(int d) { return d == 128 ? 256 : 128; }  // of a work item
+__host__ __device__ constexpr int pt_bk(int d) { return d == 128 ? 128 : 64; }     // keys of a block (32 KB)
 
-// MN-major shared-memory operand with the 128-byte swizzle: 64-element runs along N, 8 K-rows per 1024-byte group; [16,30) leading
-// byte offset >> 4 = distance between 64-wide N chunks, [32,46) stride byte offset >> 4 = distance between 8-row K groups.
-__device__ __forceinline__ uint64_t pt_desc_mn(uint32_t smem_addr, uint32_t chunk_bytes) {
-  return static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4) | static_cast<uint64_t>(chunk_bytes >> 4) << 16 | static_cast<uint64_t>(1024 >> 4) << 32 |
-         static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
-}
 __device__ __forceinline__ float pt_max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -600,15 +628,17 @@ struct __align__(16) PtPiece {
   int part;         // 0 = the whole tile: the output; else 1 + which of the CTA's two partial tiles
   int pad[2];
 };
-constexpr int PT_PIECES = 4;
+constexpr int PT_PIECES = 4;  // (the barriers below come in fours)
 
 struct __align__(16) PtBars {
   PtPiece piece[PT_PIECES];
   uint64_t piece_full[PT_PIECES], piece_read[PT_PIECES];
-  uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[4];     // pair: per tile; wide: per score buffer
-  uint64_t p_full[2][4];  // pair: per tile and 32 keys; wide: [0] per score buffer
-  uint64_t done[4];       // pair: per tile, its last product has landed; wide: per score buffer, the block's product has
+  uint64_t q_full, q_empty;      // the queries of a tile have landed in shared memory; may be overwritten there
+  uint64_t q_in, q_used;         // wide: they are in tensor memory; may be overwritten there
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[2];            // pair: per tile; wide: per score buffer
+  uint64_t p_full[2][4];         // the same, and 32 of the block's keys
+  uint64_t done[4];              // pair: per tile, its last product has landed; wide: [block % 4], the block's product has
   uint64_t o_free;        // wide: the output of a tile has been read
   uint64_t pub[2][4];     // wide: per group and warp: the reference maximum after this block; at the end of a tile, its sums
   uint64_t fin[2][4];
@@ -638,18 +668,54 @@ struct PtReader {
   }
 };
 
-// The walk over the CTA's share, and its queries: `tiles` of `rows` rows each (128 / ratio * ratio) per piece.  Leaves the header for the
-// joining kernel behind.
+// Several barriers in the time of one: a wait is a round trip of a hundred clocks even where the phase has passed, and lanes can ask for
+// different ones.
+struct PtWait {
+  uint64_t* bar;
+  uint32_t parity;
+};
+__device__ __forceinline__ bool pt_wait(const PtWait& a, const PtWait& b, const PtWait& c, volatile int* abort_flag) {
+  const int which = threadIdx.x & 3;
+  return __all_sync(0xffffffffu, wait_or_abort(which == 0 ? a.bar : which == 1 ? b.bar : c.bar, which == 0 ? a.parity : which == 1 ? b.parity : c.parity, abort_flag));
+}
+
+// Products whose descriptors differ in the low word only (start address, leading offset): the high word (stride 1024 bytes, version,
+// 128-byte swizzle) is a constant.
+constexpr uint32_t PT_DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t pt_desc_lo(uint32_t smem_addr, uint32_t chunk_bytes) { return (smem_addr & 0x3FFFF) >> 4 | chunk_bytes >> 4 << 16; }
+__device__ __forceinline__ void pt_mma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(PT_DESC_HI)
+      : "memory");
+}
+__device__ __forceinline__ void pt_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(PT_DESC_HI)
+      : "memory");
+}
+
+// The same value in every lane, known to the compiler as such (a reduction ends in a uniform register).  The operands of the tensor-core
+// instructions are uniform registers: from values that only happen to agree, each instruction pays for moving its own.
+__device__ __forceinline__ int pt_uniform(int x) { return static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<uint32_t>(x))); }
+
+// The walk over the CTA's share, and its queries: one or two tiles of whole tokens per piece.  Leaves the header for the joining kernel
+// behind.
 template <int D>
-__device__ __forceinline__ void pt_lead(const PagedAttnParams& p, const long long* prefix, long long tiles, const CUtensorMap* map, uint8_t* sq, PtBars& bars) {
-  constexpr int NCH = D / 64, CH = 16384;
-  const int lane = threadIdx.x & 31, half = 128 / p.ratio * p.ratio, tokens = 128 / p.ratio;
-  PaPlace at{};
-  const PaShare share = pa_share<pt_bk(D)>(p, prefix, tiles, at);
+__device__ __forceinline__ void pt_lead(const PagedAttnParams& p, PaPlace at, const PaShare& share, const CUtensorMap* map, uint8_t* sq, PtBars& bars) {
+  constexpr int NCH = D / 64, CH = 16384, TILES = pt_rows(D) / 128;
+  const int lane = threadIdx.x & 31, tokens = p.tile_tokens / TILES, half = tokens * p.ratio;
   int4 header = make_int4(0, 0, 0, 0);
   uint32_t n = 0, queries = 0;
   bool ok = true;
-  long long x = share.x0;
+  uint32_t x = share.x0;
   while (true) {
     const uint32_t s = n % PT_PIECES;
     if (n >= PT_PIECES) ok = __all_sync(0xffffffffu, wait_or_abort(&bars.piece_read[s], (n / PT_PIECES - 1) & 1, &bars.abort));
@@ -657,12 +723,12 @@ __device__ __forceinline__ void pt_lead(const PagedAttnParams& p, const long lon
     const bool any = x < share.x1;
     PtPiece w{};
     if (any) {
-      const int first = at.tile * p.tile_rows / p.ratio;
+      const int first = at.tile * p.tile_tokens;
       w.rows = min(p.tile_rows, at.r.n * p.ratio - at.tile * p.tile_rows);
       w.b = at.b;
       w.g = at.g;
       w.blk = at.blk;
-      w.end = static_cast<int>(min(static_cast<long long>(at.nblk), at.blk + (share.x1 - x)));
+      w.end = static_cast<int>(min(static_cast<uint32_t>(at.nblk), at.blk + (share.x1 - x)));
       w.len = at.r.len;
       w.seen = p.causal ? at.r.len - at.r.n + first + 1 : at.r.len;
       w.step = p.causal;
@@ -693,10 +759,15 @@ __device__ __forceinline__ void pt_lead(const PagedAttnParams& p, const long lon
   if (lane == 0) reinterpret_cast<int4*>(p.ws)[blockIdx.x] = header;
 }
 
-// Keys or values of the share: one block after the other into a ring of two.  A block's boxes: lane = piece of the block * chunks +
-// chunk of 64 channels.  Stays until its last copies have landed.
-template <int D>
-__device__ __forceinline__ void pt_stream(const PagedAttnParams& p, const CUtensorMap* map, uint8_t* ring, uint64_t* full, uint64_t* empty, PtBars& bars) {
+// Keys (values) of the share: one block after the other into a ring of two.  A block's boxes: lane = piece of the block * chunks + chunk of
+// 64 channels.  A warp may look after both rings.  Stays until its last copies have landed.
+struct PtRing {
+  const CUtensorMap* map;
+  uint8_t* at;
+  uint64_t *full, *empty;
+};
+template <int D, int N>
+__device__ __forceinline__ void pt_stream(const PagedAttnParams& p, const PtRing (&rings)[N], PtBars& bars) {
   constexpr int BK = pt_bk(D), NCH = D / 64, BYTES = BK * D * 2;
   const int lane = threadIdx.x & 31, rows = min(BK, 1 << p.page_shift), chunk = lane % NCH, row = lane / NCH * rows;
   // This lane's page of block j: -1 where nothing is to be copied, P (out of the map's bounds: zeros) for a bad number.
@@ -710,29 +781,32 @@ __device__ __forceinline__ void pt_stream(const PagedAttnParams& p, const CUtens
     }
     return n;
   };
-  uint32_t i = 0;
+  uint32_t blocks[N] = {}, i = 0;  // blocks requested per ring; blocks begun
   bool ok = true;
   PtReader reader;
   PtPiece at{};
   while (ok && reader.next(bars, at)) {
     int page = page_of(at, at.blk);
 #pragma unroll 1
-    for (int j = at.blk; j < at.end; ++j, ++i) {
-      const int now = page, s = i & 1;
+    for (int j = at.blk; j < at.end && ok; ++j, ++i) {
+      const int now = page, s = i & 1, off = (j * BK + row) & ((1 << p.page_shift) - 1);
       if (j + 1 < at.end) page = page_of(at, j + 1);
-      if (i >= 2 && !__all_sync(0xffffffffu, wait_or_abort(&empty[s], ((i >> 1) & 1) ^ 1, &bars.abort))) {
-        ok = false;
-        break;
+      const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, now >= 0)) * rows * 128, par = ((i >> 1) & 1) ^ 1;
+#pragma unroll
+      for (int r = 0; r < N; ++r) {
+        if (i >= 2) ok = ok && __all_sync(0xffffffffu, wait_or_abort(&rings[r].empty[s], par, &bars.abort));
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&rings[r].full[s], bytes);
+        __syncwarp();
+        if (now >= 0) tma_load_4d(rings[r].at + s * BYTES + chunk * (BK * 128) + row * 128, rings[r].map, &rings[r].full[s], chunk * 64, off, at.g, now);
+        blocks[r] = i + 1;
       }
-      const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, now >= 0));
-      if (lane == 0) mbar_arrive_expect_tx(&full[s], boxes * rows * 128);
-      __syncwarp();
-      if (now >= 0)
-        tma_load_4d(ring + s * BYTES + chunk * (BK * 128) + row * 128, map, &full[s], chunk * 64, (j * BK + row) & ((1 << p.page_shift) - 1), at.g, now);
     }
   }
   __syncwarp();
-  for (uint32_t k = i < 2 ? 0 : i - 2; k < i; ++k) mbar_wait(&full[k & 1], (k >> 1) & 1);
+#pragma unroll
+  for (int r = 0; r < N; ++r)
+    for (uint32_t k = blocks[r] < 2 ? 0 : blocks[r] - 2; k < blocks[r]; ++k) mbar_wait(&rings[r].full[k & 1], (k >> 1) & 1);
 }
 
 // Zero the values of block j that lie behind the request's last key.  By a whole warp, after the block has landed.
@@ -750,21 +824,53 @@ __device__ __forceinline__ void pt_clear_tail(uint8_t* block, int len, int j) {
   __syncwarp();
 }
 
-// 32 finished or partial channels of a row.
-__device__ __forceinline__ void pt_store32(const PagedAttnParams& p, float* part, long long at, const uint32_t (&o)[32], float inv) {
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[8 * k + e]) * inv;
-    if (part) {
-      float4* dst = reinterpret_cast<float4*>(part + 8 * k);
-      dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-      dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      pa_store8(p, at + 8 * k, v);
-    }
+// 32 bytes of registers (r[first] ..) to global memory: one 256-bit store, or two of 128 bits where the caller's tensor is
+// only 16-byte aligned.
+template <int N>
+__device__ __forceinline__ void pt_store_32b(void* dst, const uint32_t (&r)[N], int first, int wide) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(r[first]), "r"(r[first + 1]), "r"(r[first + 2]),
+                 "r"(r[first + 3]), "r"(r[first + 4]), "r"(r[first + 5]), "r"(r[first + 6]), "r"(r[first + 7])
+                 : "memory");
+  } else {
+    uint4* d = static_cast<uint4*>(dst);
+    d[0] = make_uint4(r[first], r[first + 1], r[first + 2], r[first + 3]);
+    d[1] = make_uint4(r[first + 4], r[first + 5], r[first + 6], r[first + 7]);
   }
+}
+// 32 channels of a finished row, `at` elements into the output: whole 32-byte sectors straight from a thread's registers.
+__device__ __forceinline__ void pt_store32(const PagedAttnParams& p, long long at, const uint32_t (&o)[32], float inv) {
+  uint32_t ob[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) ob[e] = pack_bf16(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+  if (p.out) {
+    pt_store_32b(p.out + at, ob, 0, p.wide_out);
+    pt_store_32b(p.out + at + 16, ob, 8, p.wide_out);
+  }
+  if (p.out_planes) {
+    uint32_t w[3][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float x[4];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&ob[2 * e + k]));
+        x[2 * k] = f.x * p.plane_scale;
+        x[2 * k + 1] = f.y * p.plane_scale;
+      }
+      split3_quad(x, w[0][e], w[1][e], w[2][e]);
+    }
+    const long long plane = static_cast<long long>(p.T) * p.ld_out;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) pt_store_32b(p.out_planes + k * plane + at, w[k], 0, p.wide_out);
+  }
+}
+// A partial tile in the workspace: four channels of 128 rows side by side, so that a warp's rows are one run: float4 number
+// (64-column order) [column / 4][row].
+__device__ __forceinline__ void pt_part32(float4* part, int column, int row, const uint32_t (&o)[32]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    part[(column / 4 + e) * 128 + row] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
 }
 
 // Masks, maximum, exponentials and the bf16 weights of N words of 32 scores of one row; `seen` keys of them count.
@@ -808,30 +914,42 @@ __device__ __forceinline__ void pt_rescale(uint32_t t_o, int words, float f) {
   tc_wait_st();
 }
 
-// Set-up that both tile forms share: barriers, tensor memory, the line of key blocks.
+// Set-up that both tile forms share: barriers, tensor memory, and (warp 3) the CTA's share.
 template <int D>
-__device__ __forceinline__ long long pt_begin(const PagedAttnParams& p, PtBars& bars, long long* prefix) {
+__device__ __forceinline__ PaShare pt_begin(const PagedAttnParams& p, PtBars& bars, const CUtensorMap* q, const CUtensorMap* k, const CUtensorMap* v, PaPlace& first) {
   const int tid = threadIdx.x, warp = tid >> 5;
+  PaShare share{};
+  if (warp == 3) {
+    if (p.pdl) pdl_wait();
+    share = pa_share<pt_bk(D)>(p, first);
+  }
   if (tid == 0) {
-    for (int i = 0; i < PT_PIECES; ++i) {
+    tma_prefetch_desc(q);
+    tma_prefetch_desc(k);
+    tma_prefetch_desc(v);
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&bars.piece_full[i], 1);
       mbar_init(&bars.piece_read[i], 11);  // eight softmax warps, keys, values, products
-      mbar_init(&bars.s_full[i], 1);
       mbar_init(&bars.done[i], 1);
+      for (int w = 0; w < 2; ++w) {
+        mbar_init(&bars.p_full[w][i], 4);
+        mbar_init(&bars.pub[w][i], 1);
+        mbar_init(&bars.fin[w][i], 1);
+      }
     }
-    mbar_init(&bars.q_full, 1);
-    mbar_init(&bars.q_empty, 1);
+#pragma unroll 1
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.s_full[i], 1);
       mbar_init(&bars.k_full[i], 1);
       mbar_init(&bars.k_empty[i], 1);
       mbar_init(&bars.v_full[i], 1);
       mbar_init(&bars.v_empty[i], 1);
-      for (int w = 0; w < 4; ++w) {
-        mbar_init(&bars.p_full[i][w], 4);
-        mbar_init(&bars.pub[i][w], 1);
-        mbar_init(&bars.fin[i][w], 1);
-      }
     }
+    mbar_init(&bars.q_full, 1);
+    mbar_init(&bars.q_empty, D == 128 ? 1 : 8);  // wide: eight warps take them to tensor memory
+    mbar_init(&bars.q_in, 8);
+    mbar_init(&bars.q_used, 1);
     mbar_init(&bars.o_free, 8);
     mbar_init(&bars.mma_done, 1);
     bars.abort = 0;
@@ -843,14 +961,54 @@ __device__ __forceinline__ long long pt_begin(const PagedAttnParams& p, PtBars& 
   }
   if (p.pdl) {
     if (tid == 0) pdl_launch_dependents();
-    pdl_wait();
+    if (warp != 3) pdl_wait();
   }
-  pa_zero_rows<D>(p, PT_THREADS);
-  const long long tiles = pa_schedule<pt_bk(D), PT_THREADS>(p, prefix);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  return tiles;
+  return share;
+}
+
+// What a softmax warp does with N * 32 scores of a row that are in tensor memory at t_s: the block's maximum ...
+template <int N>
+__device__ __forceinline__ float pt_scores(uint32_t t_s, uint32_t (&v)[N][32], int seen, float scale) {
+  tc_fence_after();
+#pragma unroll
+  for (int w = 0; w < N; ++w) tmem_ld32(t_s + w * 32, v[w]);
+  tc_wait_ld();
+  return pt_row_max<N>(v, seen) * scale;
+}
+// ... and the weights relative to m over them, handed over 32 keys at a time (the last ones by the caller); returns their sum.
+template <int N>
+__device__ __forceinline__ float pt_probabilities(uint32_t t_s, const uint32_t (&v)[N][32], float m, uint64_t c2, uint64_t* handed) {
+  const uint64_t nm = pt_pair(-m, -m);
+  uint64_t sum[2] = {pt_pair(0.f, 0.f), pt_pair(0.f, 0.f)};
+#pragma unroll
+  for (int w = 0; w < N; ++w) {
+    uint32_t pk[16];
+    pt_weights(v[w], c2, nm, sum[w & 1], pk);
+    tmem_st16(t_s + w * 16, pk);
+    tc_wait_st();
+    if (w < N - 1) {
+      tc_fence_before();
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(&handed[w]);
+    }
+  }
+  float a0, a1;
+  pt_unpair(pt_add2(sum[0], sum[1]), a0, a1);
+  return a0 + a1;
+}
+// Hands over the last weights of a block; all of them in a warp without query rows.
+template <int N>
+__device__ __forceinline__ void pt_hand_over(bool live, uint64_t* handed) {
+  tc_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) {
+    if (!live)
+      for (int w = 0; w < N - 1; ++w) mbar_arrive(&handed[w]);
+    mbar_arrive(&handed[N - 1]);
+  }
 }
 
 __global__ void __launch_bounds__(PT_THREADS, 1)
@@ -858,23 +1016,23 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                   const PagedAttnParams p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ PtBars bars;
-  constexpr int D = 128, BK = 128, KV = 32768, CH = 16384;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int D = 128, BK = pt_bk(D), KV = 32768, CH = 16384;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sq = smem, *sk = smem + 65536, *sv = sk + 2 * KV;
-  long long* prefix = reinterpret_cast<long long*>(smem + PT_SMEM - 1024);
-  const long long tiles = pt_begin<D>(p, bars, prefix);
-  const uint32_t tmem = bars.tmem_base;  // S / P of tile t at 128 t, O of tile t at 256 + 128 t
+  PaPlace first{};
+  const PaShare share = pt_begin<D>(p, bars, &tm_q, &tm_k, &tm_v, first);
+  constexpr uint32_t tmem = 0;           // all 512 columns are this CTA's: S / P of tile t at 128 t, O of tile t at 256 + 128 t
   const int half = p.tile_rows >> 1;     // rows of a tile
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_CONTROL));
-    if (warp == 0) {
-      pt_stream<D>(p, &tm_k, sk, bars.k_full, bars.k_empty, bars);
-    } else if (warp == 2) {
-      pt_stream<D>(p, &tm_v, sv, bars.v_full, bars.v_empty, bars);
-    } else if (warp == 3) {
-      pt_lead<D>(p, prefix, tiles, &tm_q, sq, bars);
+    if (warp == 3) {
+      pt_lead<D>(p, first, share, &tm_q, sq, bars);
+    } else if (warp != 1) {
+      const bool k = warp == 0;
+      const PtRing rings[1] = {{k ? &tm_k : &tm_v, k ? sk : sv, k ? bars.k_full : bars.v_full, k ? bars.k_empty : bars.v_empty}};
+      pt_stream<D, 1>(p, rings, bars);
     } else {
       const bool leader = elect_one();
       const uint32_t idesc_s = idesc_bf16_f32(128, BK) | p.negate_q, idesc_o = idesc_bf16_f32(128, D) | (1u << 16);
@@ -886,58 +1044,59 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       uint32_t i = 0, i_second = 0;  // blocks so far, and those with a second tile
       PtReader reader;
       PtPiece at{};
-      auto piece = [&] {
-        const int nt = at.rows > half ? 2 : 1, end = at.end;
-        const uint32_t n = reader.n - 1;
-        auto issue_s = [&](int t, uint32_t block) {
-          const uint64_t qd = smem_desc_sw128(smem_u32(sq + t * 32768)), kd = smem_desc_sw128(smem_u32(sk + (block & 1) * KV));
-#pragma unroll
-          for (int ks = 0; ks < 8; ++ks) {
-            const uint32_t o = (ks >> 2) * (CH >> 4) + (ks & 3) * 2;
-            if (leader) umma_ss_bf16(tmem + t * 128, qd + o, kd + o, idesc_s, ks > 0 ? 1u : 0u);
-          }
-          if (leader) tc_commit(&bars.s_full[t]);
-        };
-        if (!wait(&bars.q_full, n & 1) || !wait(&bars.k_full[i & 1], (i >> 1) & 1)) return false;
-        tc_fence_after();
-        for (int t = 0; t < nt; ++t) issue_s(t, i);
-        if (leader) {
-          tc_commit(&bars.k_empty[i & 1]);
-          if (at.blk + 1 == end) tc_commit(&bars.q_empty);
-        }
-        __syncwarp();
+      while (ok && reader.next(bars, at)) {
+        const int nt = pt_uniform(at.rows > half ? 2 : 1), nb = pt_uniform(at.end - at.blk), blk = pt_uniform(at.blk), len = pt_uniform(at.len);
+        if (!wait(&bars.q_full, (reader.n - 1) & 1)) break;
 #pragma unroll 1
-        for (int j = at.blk; j < end; ++j, ++i) {
-          const int s = i & 1;
-          const bool more = j + 1 < end;
-          if (!wait(&bars.v_full[s], (i >> 1) & 1)) return false;
-          pt_clear_tail<D>(sv + s * KV, at.len, j);
-          if (more && !wait(&bars.k_full[s ^ 1], ((i + 1) >> 1) & 1)) return false;
-          const uint64_t v_desc = pt_desc_mn(smem_u32(sv + s * KV), CH);
-          for (int t = 0; t < nt; ++t) {
-            const uint32_t par = (t ? i_second : i) & 1;
-#pragma unroll
-            for (int part = 0; part < 4; ++part) {  // each 32 keys' product starts under the next ones' exponentials
-              if (!wait(&bars.p_full[t][part], par)) return false;
+        for (int j = -1; j < nb && ok; ++j) {
+          const bool more = j + 1 < nb;
+          const uint32_t vb = i + j, kb = i + j + 1;  // blocks of this product and of the scores after it
+          const uint32_t v_desc = pt_desc_lo(smem_u32(sv + (vb & 1) * KV), CH), k_desc = pt_desc_lo(smem_u32(sk + (kb & 1) * KV), 16);
+          const PtWait keys{&bars.k_full[kb & 1], (kb >> 1) & 1}, values{&bars.v_full[vb & 1], (vb >> 1) & 1};
+#pragma unroll 1
+          for (int t = 0; t < nt && ok; ++t) {
+            if (j < 0) {
+              ok = t > 0 || wait(keys.bar, keys.parity);
               tc_fence_after();
+            } else {
+              const PtWait weights{&bars.p_full[t][0], ((t ? i_second : i) + j) & 1};
+              ok = t ? wait(weights.bar, weights.parity) : pt_wait(values, weights, more ? keys : values, &bars.abort);
+              if (!ok) break;
+              tc_fence_after();
+              if (t == 0) pt_clear_tail<D>(sv + (vb & 1) * KV, len, blk + j);
 #pragma unroll
-              for (int ks = 2 * part; ks < 2 * part + 2; ++ks)
-                if (leader) umma_ts_bf16(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, v_desc + ks * (2048 >> 4), idesc_o, j > at.blk || ks ? 1u : 0u);
+              for (int part = 0; part < 4; ++part) {  // each 32 keys' product starts under the next ones' exponentials
+                if (part) {
+                  if (!wait(&bars.p_full[t][part], weights.parity)) break;
+                  tc_fence_after();
+                }
+#pragma unroll
+                for (int ks = 2 * part; ks < 2 * part + 2; ++ks)
+                  if (leader) pt_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, v_desc + ks * (2048 >> 4), idesc_o, j > 0 || ks ? 1u : 0u);
+              }
             }
-            if (more) issue_s(t, i + 1);
-            else if (leader) tc_commit(&bars.done[t]);
+            if (!ok) break;
+            if (more) {
+              const uint32_t q_desc = pt_desc_lo(smem_u32(sq + t * 32768), 16);
+#pragma unroll
+              for (int ks = 0; ks < 8; ++ks) {
+                const uint32_t o = (ks >> 2) * (CH >> 4) + (ks & 3) * 2;
+                if (leader) pt_mma_ss(tmem + t * 128, q_desc + o, k_desc + o, idesc_s, ks > 0 ? 1u : 0u);
+              }
+              if (leader) tc_commit(&bars.s_full[t]);
+            } else if (leader) {
+              tc_commit(&bars.done[t]);
+            }
           }
-          if (leader) {
-            tc_commit(&bars.v_empty[s]);
-            if (more) tc_commit(&bars.k_empty[s ^ 1]);
-            if (j + 2 == end) tc_commit(&bars.q_empty);
+          if (ok && leader) {
+            if (more) tc_commit(&bars.k_empty[kb & 1]);
+            if (j + 2 == nb) tc_commit(&bars.q_empty);  // the last scores have been issued
+            if (j >= 0) tc_commit(&bars.v_empty[vb & 1]);
           }
           __syncwarp();
-          if (nt == 2) ++i_second;
         }
-        return true;
-      };
-      while (reader.next(bars, at) && piece()) {
+        i += nb;
+        if (nt == 2) i_second += nb;
       }
       ok = ok && reader.ok;
       // nothing of this CTA's tensor work may be in flight when it gives up its tensor memory
@@ -956,6 +1115,8 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const uint32_t t_s = tmem + t * 128 + lane_addr, t_o = tmem + 256 + t * 128 + lane_addr;
     const uint64_t c2 = pt_pair(p.abs_scale_log2e, p.abs_scale_log2e);
     const int local = t * half + row, ahead = local / p.ratio;  // row of the piece; its token's number in it
+    pa_check(p, tid - 128, 256);
+    pa_zero_rows<D>(p, tid - 128, 256);
     uint32_t n = 0, i = 0;  // tiles and blocks of this group
     bool ok = true;
     PtReader reader;
@@ -971,12 +1132,8 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         ok = __all_sync(0xffffffffu, wait_or_abort(&bars.s_full[t], i & 1, &bars.abort, p.wait_limit));
         if (!ok) break;
         if (live) {
-          tc_fence_after();
           uint32_t v[4][32];
-#pragma unroll
-          for (int w = 0; w < 4; ++w) tmem_ld32(t_s + w * 32, v[w]);
-          tc_wait_ld();
-          const float m_blk = pt_row_max<4>(v, limit - j * BK) * p.abs_scale_log2e;
+          const float m_blk = pt_scores<4>(t_s, v, limit - j * BK, p.abs_scale_log2e);
           const bool grow = m_blk > m_ref + PT_RESCALE;
           if (__any_sync(0xffffffffu, grow)) {
             if (j > at.blk) {  // the scores of this block came after the last one's product
@@ -986,50 +1143,30 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             }
             if (grow) m_ref = m_blk;
           }
-          const uint64_t nm = pt_pair(-m_ref, -m_ref);
-          uint64_t sum[2] = {pt_pair(0.f, 0.f), pt_pair(0.f, 0.f)};
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            uint32_t pk[16];
-            pt_weights(v[w], c2, nm, sum[w & 1], pk);
-            tmem_st16(t_s + w * 16, pk);
-            tc_wait_st();
-            if (w < 3) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&bars.p_full[t][w]);
-            }
-          }
-          float a0, a1;
-          pt_unpair(pt_add2(sum[0], sum[1]), a0, a1);
-          l += a0 + a1;
+          l += pt_probabilities<4>(t_s, v, m_ref, c2, bars.p_full[t]);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if (!live)
-            for (int w = 0; w < 3; ++w) mbar_arrive(&bars.p_full[t][w]);
-          mbar_arrive(&bars.p_full[t][3]);
-        }
+        pt_hand_over<4>(live, bars.p_full[t]);
       }
       ok = ok && __all_sync(0xffffffffu, wait_or_abort(&bars.done[t], n & 1, &bars.abort));
       ++n;
       if (ok && live) {
         tc_fence_after();
         const float inv = at.part ? 1.f : l == 0.f ? 0.f : 1.f / l;
-        float* part = !at.part ? nullptr
-                               : reinterpret_cast<float*>(p.ws + pa_header_bytes(gridDim.x) + (2ll * blockIdx.x + at.part - 1) * pa_part_bytes<pt_rows(D), D>());
+        // [tile][column / 4][row], then the references and sums of both tiles
+        float4* part = reinterpret_cast<float4*>(p.ws + pa_header_bytes(gridDim.x) + (2ll * blockIdx.x + at.part - 1) * pa_part_bytes<pt_rows(D), D>());
         const long long to = static_cast<long long>(at.token + ahead) * p.ld_out + static_cast<long long>(at.g * p.ratio + local - ahead * p.ratio) * D;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
           tmem_ld32(t_o + c * 32, o);
           tc_wait_ld();
-          if (mine) pt_store32(p, part ? part + local * D + c * 32 : nullptr, to + c * 32, o, inv);
+          if (at.part) pt_part32(part + t * (D / 4) * 128, c * 32, row, o);
+          else if (mine) pt_store32(p, to + c * 32, o, inv);
         }
-        if (part && mine) {
-          part[pt_rows(D) * D + local] = m_ref;
-          part[pt_rows(D) * D + pt_rows(D) + local] = l;
+        if (at.part) {
+          float* stat = reinterpret_cast<float*>(part + pt_rows(D) * D / 4);
+          stat[t * 128 + row] = m_ref;
+          stat[pt_rows(D) + t * 128 + row] = l;
         }
         tc_fence_before();
       }
@@ -1053,22 +1190,22 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                   const PagedAttnParams p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ PtBars bars;
-  constexpr int D = 256, BK = 64, KV = 32768, QCH = 16384, CH = 8192, AHEAD = 3;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int D = 256, BK = pt_bk(D), KV = 32768, QCH = 16384, CH = BK * 128;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sq = smem, *sk = smem + 65536, *sv = sk + 2 * KV;
-  long long* prefix = reinterpret_cast<long long*>(smem + PT_SMEM - 1024);
-  const long long tiles = pt_begin<D>(p, bars, prefix);
-  const uint32_t tmem = bars.tmem_base;  // score buffers of 64 columns at 0, 64, 128, 192, O at 256
+  PaPlace first{};
+  const PaShare share = pt_begin<D>(p, bars, &tm_q, &tm_k, &tm_v, first);
+  constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's: two score buffers of 64 columns, queries from 128 (two channels a column), O from 256
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_CONTROL));
-    if (warp == 0) {
-      pt_stream<D>(p, &tm_k, sk, bars.k_full, bars.k_empty, bars);
-    } else if (warp == 2) {
-      pt_stream<D>(p, &tm_v, sv, bars.v_full, bars.v_empty, bars);
-    } else if (warp == 3) {
-      pt_lead<D>(p, prefix, tiles, &tm_q, sq, bars);
+    if (warp == 3) {
+      pt_lead<D>(p, first, share, &tm_q, sq, bars);
+    } else if (warp != 1) {
+      const bool k = warp == 0;
+      const PtRing rings[1] = {{k ? &tm_k : &tm_v, k ? sk : sv, k ? bars.k_full : bars.v_full, k ? bars.k_empty : bars.v_empty}};
+      pt_stream<D, 1>(p, rings, bars);
     } else {
       const bool leader = elect_one();
       const uint32_t idesc_s = idesc_bf16_f32(128, BK) | p.negate_q, idesc_o = idesc_bf16_f32(128, D) | (1u << 16);
@@ -1077,56 +1214,57 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         ok = ok && __all_sync(0xffffffffu, wait_or_abort(bar, parity, &bars.abort));
         return ok;
       };
-      const uint64_t qd = smem_desc_sw128(smem_u32(sq));
       uint32_t i = 0;  // blocks so far
       PtReader reader;
       PtPiece at{};
       while (ok && reader.next(bars, at)) {
         const uint32_t n = reader.n - 1;
-        auto issue_s = [&](uint32_t block) {
-          if (!wait(&bars.k_full[block & 1], (block >> 1) & 1)) return;
+        const int nb = pt_uniform(at.end - at.blk), blk = pt_uniform(at.blk), len = pt_uniform(at.len);
+        if (!wait(&bars.q_in, n & 1)) break;
+#pragma unroll 1
+        for (int j = -2; j < nb; ++j) {
+          const bool more = j + 2 < nb;
+          const uint32_t vb = i + j, kb = i + j + 2, s = vb & 1;  // blocks of this product and of the scores after it, their buffer
+          const PtWait keys{&bars.k_full[s], (kb >> 1) & 1}, values{&bars.v_full[s], (vb >> 1) & 1};
+          if (j == 0 && n > 0 && !wait(&bars.o_free, (n - 1) & 1)) break;  // the last tile's output has been read
+          ok = j < 0 ? !more || wait(keys.bar, keys.parity) : pt_wait(values, {&bars.p_full[s][0], (vb >> 1) & 1}, more ? keys : values, &bars.abort);
+          if (!ok) break;
           tc_fence_after();
-          const uint64_t kd = smem_desc_sw128(smem_u32(sk + (block & 1) * KV));
+          if (j >= 0) {
+            pt_clear_tail<D>(sv + s * KV, len, blk + j);
+            const uint32_t v_desc = pt_desc_lo(smem_u32(sv + s * KV), CH);
 #pragma unroll
-          for (int ks = 0; ks < 16; ++ks) {
-            const uint32_t qo = (ks >> 2) * (QCH >> 4) + (ks & 3) * 2, ko = (ks >> 2) * (CH >> 4) + (ks & 3) * 2;
-            if (leader) umma_ss_bf16(tmem + (block & 3) * 64, qd + qo, kd + ko, idesc_s, ks > 0 ? 1u : 0u);
+            for (int part = 0; part < 2; ++part) {  // the first 32 keys' product starts under the others' exponentials
+              if (part) {
+                if (!wait(&bars.p_full[s][1], (vb >> 1) & 1)) break;
+                tc_fence_after();
+              }
+#pragma unroll
+              for (int ks = 2 * part; ks < 2 * part + 2; ++ks)
+                if (leader) pt_mma_ts(tmem + 256, tmem + s * 64 + ks * 8, v_desc + ks * (2048 >> 4), idesc_o, j > 0 || ks ? 1u : 0u);
+            }
+            if (!ok) break;
+          }
+          if (more) {
+            const uint32_t k_desc = pt_desc_lo(smem_u32(sk + s * KV), 16);
+#pragma unroll
+            for (int ks = 0; ks < 16; ++ks) {
+              const uint32_t o = (ks >> 2) * (CH >> 4) + (ks & 3) * 2;
+              if (leader) pt_mma_ts(tmem + s * 64, tmem + 128 + ks * 8, k_desc + o, idesc_s, ks > 0 ? 1u : 0u);
+            }
           }
           if (leader) {
-            tc_commit(&bars.k_empty[block & 1]);
-            tc_commit(&bars.s_full[block & 3]);
+            if (more) {
+              tc_commit(&bars.s_full[s]);
+              tc_commit(&bars.k_empty[s]);
+              if (j + 3 == nb) tc_commit(&bars.q_used);  // the last scores have been issued
+            }
+            if (j >= 0) {
+              tc_commit(&bars.done[vb & 3]);
+              tc_commit(&bars.v_empty[s]);
+            }
           }
           __syncwarp();
-        };
-        const int nb = at.end - at.blk;
-        if (!wait(&bars.q_full, n & 1)) break;
-#pragma unroll 1
-        for (int j = -AHEAD; j < nb && ok; ++j) {
-          if (j >= 0) {
-            const uint32_t block = i + j;
-            const int s = block & 1;
-            if (j == 0 && n > 0 && !wait(&bars.o_free, (n - 1) & 1)) break;  // the last tile's output has been read
-            if (!wait(&bars.v_full[s], (block >> 1) & 1)) break;
-            pt_clear_tail<D>(sv + s * KV, at.len, at.blk + j);
-            if (!wait(&bars.p_full[0][block & 3], (block >> 2) & 1)) break;
-            tc_fence_after();
-            const uint64_t v_desc = pt_desc_mn(smem_u32(sv + s * KV), CH);
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              if (leader) umma_ts_bf16(tmem + 256, tmem + (block & 3) * 64 + ks * 8, v_desc + ks * (2048 >> 4), idesc_o, j > 0 || ks ? 1u : 0u);
-            if (leader) {
-              tc_commit(&bars.v_empty[s]);
-              tc_commit(&bars.done[block & 3]);
-            }
-            __syncwarp();
-          }
-          if (j + AHEAD < nb) {
-            issue_s(i + j + AHEAD);
-            if (ok && j + AHEAD == nb - 1) {
-              if (leader) tc_commit(&bars.q_empty);
-              __syncwarp();
-            }
-          }
         }
         i += nb;
       }
@@ -1143,7 +1281,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_REGS_SOFTMAX));
     const int grp = (warp - 4) >> 2, q = warp & 3, row = q * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
-    const uint32_t t_o = tmem + 256 + lane_addr;
+    const uint32_t t_o = tmem + 256 + lane_addr, t_s = tmem + grp * 64 + lane_addr;
     const uint64_t c2 = pt_pair(p.abs_scale_log2e, p.abs_scale_log2e);
     const int ahead = row / p.ratio;  // number of the row's token in the tile
     uint32_t i = 0;                   // blocks so far (of both groups)
@@ -1152,32 +1290,55 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       ok = ok && __all_sync(0xffffffffu, wait_or_abort(bar, parity, &bars.abort));
       return ok;
     };
+    // this thread's half of its query row (two chunks of 64 channels) of tile n, from shared to tensor memory
+    auto queries = [&](uint32_t n) {
+      if (!wait(&bars.q_full, n & 1) || (n > 0 && !wait(&bars.q_used, (n - 1) & 1))) return false;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t v[32];
+        const uint8_t* src = sq + (2 * grp + c) * QCH + row * 128;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint4 x = *reinterpret_cast<const uint4*>(src + ((e ^ (row & 7)) << 4));
+          v[4 * e] = x.x;
+          v[4 * e + 1] = x.y;
+          v[4 * e + 2] = x.z;
+          v[4 * e + 3] = x.w;
+        }
+        tmem_st32(tmem + 128 + (2 * grp + c) * 32 + lane_addr, v);
+      }
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&bars.q_in);
+        mbar_arrive(&bars.q_empty);
+      }
+      return true;
+    };
     PtReader reader;
-    PtPiece at{};
-    auto piece = [&] {
-      const uint32_t n = reader.n - 1;
+    PtPiece at{}, next{};
+    bool any = reader.next(bars, at) && queries(0);
+    pa_check(p, tid - 128, 256);
+    pa_zero_rows<D>(p, tid - 128, 256);
+#pragma unroll 1
+    for (uint32_t n = 0; any; ++n) {
       const bool live = q * 32 < at.rows, mine = row < at.rows;
       const int limit = at.seen + ahead * at.step;
       float m_own = -1e30f, l = 0.f;  // the reference that l is relative to
 #pragma unroll 1
       for (int j = at.blk; j < at.end; ++j, ++i) {
         if ((i & 1) != static_cast<uint32_t>(grp)) continue;
-        const uint32_t buf = i & 3;
-        if (!__all_sync(0xffffffffu, wait_or_abort(&bars.s_full[buf], (i >> 2) & 1, &bars.abort, p.wait_limit))) return ok = false;
+        ok = __all_sync(0xffffffffu, wait_or_abort(&bars.s_full[grp], (i >> 1) & 1, &bars.abort, p.wait_limit));
+        if (!ok) break;
         uint32_t v[2][32];
         float m_blk = 0.f;
-        const uint32_t t_s = tmem + buf * 64 + lane_addr;
-        if (live) {
-          tc_fence_after();
-#pragma unroll
-          for (int w = 0; w < 2; ++w) tmem_ld32(t_s + w * 32, v[w]);
-          tc_wait_ld();
-          m_blk = pt_row_max<2>(v, limit - j * BK) * p.abs_scale_log2e;
-        }
+        if (live) m_blk = pt_scores<2>(t_s, v, limit - j * BK, p.abs_scale_log2e);
         // the reference after the block before, which the other group has
         float m_ref = -1e30f;
         if (j > at.blk) {
-          if (!wait(&bars.pub[grp ^ 1][q], ((i - 1) >> 1) & 1)) return false;
+          if (!wait(&bars.pub[grp ^ 1][q], ((i - 1) >> 1) & 1)) break;
           m_ref = bars.m_ref[grp ^ 1][row];
         }
         const bool grow = live && m_blk > m_ref + PT_RESCALE;
@@ -1187,64 +1348,52 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (lane == 0) mbar_arrive(&bars.pub[grp][q]);
         if (live) {
           if (__any_sync(0xffffffffu, grow) && j > at.blk) {
-            // The product before must have landed.  (This block's scores came after that of block i - 3, so the barrier's phase
-            // before has passed, and its next waits for this block's weights.)
-            if (!wait(&bars.done[(i - 1) & 3], ((i - 1) >> 2) & 1)) return false;
+            // The product before must have landed.  (These scores came after that of two blocks ago, so the barrier's phase before has
+            // passed, and its next waits for this block's weights.)
+            if (!wait(&bars.done[(i - 1) & 3], ((i - 1) >> 2) & 1)) break;
             tc_fence_after();
             pt_rescale(t_o, 8, grow ? pa_exp2(m_ref - m_blk) : 1.0f);
           }
-          l *= pa_exp2(m_own - m_new);
+          l = l * pa_exp2(m_own - m_new) + pt_probabilities<2>(t_s, v, m_new, c2, bars.p_full[grp]);
           m_own = m_new;
-          const uint64_t nm = pt_pair(-m_new, -m_new);
-          uint64_t sum[2] = {pt_pair(0.f, 0.f), pt_pair(0.f, 0.f)};
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            uint32_t pk[16];
-            pt_weights(v[w], c2, nm, sum[w], pk);
-            tmem_st16(t_s + w * 16, pk);
-          }
-          float a0, a1;
-          pt_unpair(pt_add2(sum[0], sum[1]), a0, a1);
-          l += a0 + a1;
-          tc_wait_st();
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.p_full[0][buf]);
+        pt_hand_over<2>(live, bars.p_full[grp]);
       }
+      if (!ok) break;
       // both groups' sums, relative to the later reference
       bars.end_m[n & 1][grp][row] = m_own;
       bars.end_l[n & 1][grp][row] = l;
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.fin[grp][q]);
-      if (!wait(&bars.fin[grp ^ 1][q], n & 1)) return false;
+      any = reader.next(bars, next);
+      if (!reader.ok || (any && !queries(n + 1))) break;  // the next scores may begin
+      if (!wait(&bars.fin[grp ^ 1][q], n & 1)) break;
       const float m_other = bars.end_m[n & 1][grp ^ 1][row], m_end = fmaxf(m_own, m_other);
       l = l * pa_exp2(m_own - m_end) + bars.end_l[n & 1][grp ^ 1][row] * pa_exp2(m_other - m_end);
-      if (!wait(&bars.done[(i - 1) & 3], ((i - 1) >> 2) & 1)) return false;
+      if (!wait(&bars.done[(i - 1) & 3], ((i - 1) >> 2) & 1)) break;
       if (live) {
         tc_fence_after();
         const float inv = at.part ? 1.f : l == 0.f ? 0.f : 1.f / l;
-        float* part = !at.part ? nullptr
-                               : reinterpret_cast<float*>(p.ws + pa_header_bytes(gridDim.x) + (2ll * blockIdx.x + at.part - 1) * pa_part_bytes<pt_rows(D), D>());
+        float4* part = reinterpret_cast<float4*>(p.ws + pa_header_bytes(gridDim.x) + (2ll * blockIdx.x + at.part - 1) * pa_part_bytes<pt_rows(D), D>());
         const long long to = static_cast<long long>(at.token + ahead) * p.ld_out + static_cast<long long>(at.g * p.ratio + row - ahead * p.ratio) * D;
 #pragma unroll 1
         for (int c = 4 * grp; c < 4 * grp + 4; ++c) {
           uint32_t o[32];
           tmem_ld32(t_o + c * 32, o);
           tc_wait_ld();
-          if (mine) pt_store32(p, part ? part + row * D + c * 32 : nullptr, to + c * 32, o, inv);
+          if (at.part) pt_part32(part, c * 32, row, o);
+          else if (mine) pt_store32(p, to + c * 32, o, inv);
         }
-        if (part && mine && grp == 0) {
-          part[pt_rows(D) * D + row] = m_end;
-          part[pt_rows(D) * D + pt_rows(D) + row] = l;
+        if (at.part && grp == 0) {
+          float* stat = reinterpret_cast<float*>(part + pt_rows(D) * D / 4);
+          stat[row] = m_end;
+          stat[pt_rows(D) + row] = l;
         }
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.o_free);
-      return true;
-    };
-    while (reader.next(bars, at) && piece()) {
+      at = next;
     }
     ok = ok && reader.ok;
     if (!ok && lane == 0) {
@@ -1260,7 +1409,49 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   }
 }
 
-// Joins the parts of the tile that CTA blockIdx.x of the kernel before began; a warp per row.
+// Joins the parts of the tile that CTA blockIdx.x of a tile form began: a thread per row and 32 columns.
+template <int D>
+__global__ void __launch_bounds__(128) paged_join_tile_kernel(const PagedAttnParams p, int ctas) {
+  if (p.pdl) {
+    pdl_launch_dependents();
+    pdl_wait();
+  }
+  const int4 h = reinterpret_cast<const int4*>(p.ws)[blockIdx.x];
+  if (h.w == 0) return;
+  constexpr int ROWS = pt_rows(D), COLS = D / 32;  // grid.y = 32 columns of 128 rows
+  const PaRequest r = pa_request(p, h.x);
+  const int t = blockIdx.y / COLS, c = blockIdx.y % COLS, row = threadIdx.x, half = 128 / p.ratio * p.ratio;
+  const int local = t * half + row, grow = h.z * p.tile_rows + local;
+  if (row >= half || grow >= r.n * p.ratio) return;
+  const uint8_t* parts = p.ws + pa_header_bytes(ctas);
+  auto part = [&](int i) {  // the i-th part of the tile
+    return reinterpret_cast<const float4*>(parts + (2ll * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * pa_part_bytes<ROWS, D>());
+  };
+  auto stat = [&](int i) { return reinterpret_cast<const float*>(part(i) + ROWS * D / 4) + t * 128 + row; };
+  float top = -INFINITY;
+  for (int i = 0; i < h.w; ++i) top = fmaxf(top, *stat(i));
+  if (top == -INFINITY) top = 0.f;
+  float sum = 0.f;
+  uint32_t o[32] = {};
+#pragma unroll 1
+  for (int i = 0; i < h.w; ++i) {
+    const float f = pa_exp2(*stat(i) - top);
+    sum += f * stat(i)[ROWS];
+    const float4* src = part(i) + (t * (D / 4) + c * 8) * 128 + row;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float4 a = src[e * 128];
+      o[4 * e] = __float_as_uint(__uint_as_float(o[4 * e]) + f * a.x);
+      o[4 * e + 1] = __float_as_uint(__uint_as_float(o[4 * e + 1]) + f * a.y);
+      o[4 * e + 2] = __float_as_uint(__uint_as_float(o[4 * e + 2]) + f * a.z);
+      o[4 * e + 3] = __float_as_uint(__uint_as_float(o[4 * e + 3]) + f * a.w);
+    }
+  }
+  const int token = grow / p.ratio;
+  pt_store32(p, (r.start + token) * p.ld_out + static_cast<long long>(h.y * p.ratio + grow - token * p.ratio) * D + c * 32, o, sum == 0.f ? 0.f : 1.f / sum);
+}
+
+// The same for the sixteen-row form; a warp per row.
 template <int ROWS, int D>
 __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnParams p, int ctas) {
   if (p.pdl) {
@@ -1319,16 +1510,13 @@ static size_t pa_workspace(int D, bool tiles, int ctas) {
 }
 
 using PaRowsKernel = void(const PagedAttnParams);
-using PaTileKernel = void(const CUtensorMap, const CUtensorMap, const CUtensorMap, const PagedAttnParams);
 using PaJoinKernel = void(const PagedAttnParams, int);
 
 static int pa_set_attributes() {
   static host::DeviceCache ready;
   const int set = host::per_device(ready, [] {
     const auto smem = [](auto* kernel, int bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess; };
-    const int rows = PR_SMEM + 8 * (PA_MAX_REQUESTS + 1);
-    const int tiles = PT_SMEM + 8 * (PA_MAX_REQUESTS + 1);
-    return smem(paged_rows_kernel<128>, rows) && smem(paged_rows_kernel<256>, rows) && smem(paged_pair_kernel, tiles) && smem(paged_wide_kernel, tiles);
+    return smem(paged_rows_kernel<128>, PR_SMEM) && smem(paged_rows_kernel<256>, PR_SMEM) && smem(paged_pair_kernel, PT_SMEM) && smem(paged_wide_kernel, PT_SMEM);
   });
   return set ? TYBOK_OK : host::fail_cuda("paged_attention: shared memory");
 }
@@ -1393,8 +1581,12 @@ int tybok_paged_attention(const void* q, int64_t ldq, const void* k_pages, const
   p.wait_limit = host::epilogue_wait_limit() > 0 ? host::epilogue_wait_limit() : kWaitLimitCycles;
   p.ws = static_cast<uint8_t*>(workspace); p.status = status_word;
   p.pdl = host::pdl_enabled() ? 1 : 0;
+  p.wide_out = ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_planes)) & 31) == 0;
   const bool tiles = pa_tile_form(p.ratio, max_tokens);
   p.tile_rows = !tiles ? PR_ROWS : 128 / p.ratio * p.ratio * (D == 128 ? 2 : 1);
+  const double most_tiles = static_cast<double>(tokens) * p.ratio / p.tile_rows + B, most_blocks = static_cast<double>(table_width) * page_size / 64 + 1;
+  if (most_tiles * G * most_blocks > 4e9) return host::fail(TYBOK_ERR_ARG, "paged_attention: more than 2^32 key blocks could fall to one call");
+  p.tile_tokens = p.tile_rows % p.ratio == 0 ? p.tile_rows / p.ratio : 0;
   p.join_blocks = tiles ? (D == 128 ? 3 : 6) : 4;
   CUtensorMap tm_q, tm_k, tm_v;
   if (tiles) {
@@ -1413,24 +1605,23 @@ int tybok_paged_attention(const void* q, int64_t ldq, const void* k_pages, const
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(tiles ? PT_THREADS : PR_THREADS);
-  cfg.dynamicSmemBytes = (tiles ? PT_SMEM : PR_SMEM) + 8 * (static_cast<size_t>(B) + 1);
+  cfg.dynamicSmemBytes = tiles ? PT_SMEM : PR_SMEM;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cfg.attrs = attr;
   cfg.numAttrs = p.pdl;
   cudaError_t e;
   if (tiles) {
-    PaTileKernel* kernel = D == 256 ? paged_wide_kernel : paged_pair_kernel;
-    e = cudaLaunchKernelEx(&cfg, kernel, tm_q, tm_k, tm_v, p);
+    e = cudaLaunchKernelEx(&cfg, D == 256 ? paged_wide_kernel : paged_pair_kernel, tm_q, tm_k, tm_v, p);
   } else {
     PaRowsKernel* kernel = D == 256 ? paged_rows_kernel<256> : paged_rows_kernel<128>;
     e = cudaLaunchKernelEx(&cfg, kernel, p);
   }
   if (e != cudaSuccess) return host::fail_cuda("launch paged_attention");
   host::count_launch();
-  cfg.gridDim = dim3(ctas, tiles ? 8 : PR_ROWS / 4);
+  cfg.gridDim = dim3(ctas, tiles ? 8 : PR_ROWS / 4);  // tile forms: 128 rows x 32 columns each
   cfg.blockDim = dim3(128);
   cfg.dynamicSmemBytes = 0;
-  PaJoinKernel* join = tiles ? (D == 256 ? paged_join_kernel<pt_rows(256), 256> : paged_join_kernel<pt_rows(128), 128>)
+  PaJoinKernel* join = tiles ? (D == 256 ? paged_join_tile_kernel<256> : paged_join_tile_kernel<128>)
                              : (D == 256 ? paged_join_kernel<PR_ROWS, 256> : paged_join_kernel<PR_ROWS, 128>);
   if (cudaLaunchKernelEx(&cfg, join, p, ctas) != cudaSuccess) return host::fail_cuda("launch paged_join_kernel");
   host::count_launch();
