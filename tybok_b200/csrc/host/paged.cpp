@@ -7,6 +7,27 @@ static void need_ints(const Tensor& t, int64_t n, const char* what, const char* 
   if (!is_vector(t, at::kInt, n)) type_error(std::string(what) + ": " + name + " must be contiguous int32 [" + std::to_string(n) + "]");
 }
 
+// Tensors of one allocation, 16-byte aligned pieces of it (an allocation each would cost a call as much as its launch).
+class Pieces {
+ public:
+  explicit Pieces(const Tensor& like) : like_(like) {}
+  void add(int64_t n) { size_ += (n + 3) & ~int64_t(3); }
+  void allocate() { buf_ = at::empty({size_}, like_.options()); }
+  Tensor take(at::IntArrayRef sizes) {
+    int64_t n = 1;
+    for (const int64_t s : sizes) n *= s;
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf_.storage()), buf_.key_set(), buf_.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(at_);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    at_ += (n + 3) & ~int64_t(3);
+    return t;
+  }
+
+ private:
+  Tensor like_, buf_;
+  int64_t size_ = 0, at_ = 0;
+};
+
 using Plan = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
 
 // (lengths, table, stack, count, cu_tokens, pos, slots, missing); the first four are the given tensors themselves in place.
@@ -29,13 +50,18 @@ static Plan page_plan(const Tensor& lens, const Tensor& fresh, const Tensor& tab
   same_device(lens.device(), what, {&fresh, &table, &stack, &count, opt(finished)});
   require_cuda(lens, what);
   const c10::cuda::CUDAGuard guard(lens.device());
-  const auto ints = lens.options();
-  Tensor lens2 = in_place ? lens : at::empty({b}, ints), table2 = in_place ? table : at::empty({b, table.size(1)}, ints);
-  Tensor stack2 = in_place ? stack : at::empty({stack.numel()}, ints), count2 = in_place ? count : at::empty({1}, ints);
-  Tensor cu = at::empty({b + 1}, ints), pos = at::empty({tokens}, ints), slots = at::empty({tokens}, ints), missing = at::empty({1}, ints);
+  const int64_t width = table.size(1), pages = stack.numel();
+  Pieces mem(lens);
+  if (!in_place)
+    for (const int64_t n : {b, b * width, pages, int64_t(1)}) mem.add(n);
+  for (const int64_t n : {b + 1, tokens, tokens, int64_t(1)}) mem.add(n);
+  mem.allocate();
+  Tensor lens2 = in_place ? lens : mem.take({b}), table2 = in_place ? table : mem.take({b, width});
+  Tensor stack2 = in_place ? stack : mem.take({pages}), count2 = in_place ? count : mem.take({1});
+  Tensor cu = mem.take({b + 1}), pos = mem.take({tokens}), slots = mem.take({tokens}), missing = mem.take({1});
   const auto ip = [](const Tensor& t) { return static_cast<int*>(t.data_ptr()); };
   check(tybok_page_plan(ip(lens), ip(fresh), ptr(finished), ip(table), ip(stack), ip(count), ip(lens2), ip(table2), ip(stack2), ip(count2), ip(cu),
-                        ip(pos), ip(slots), ip(missing), b, table.size(1), stack.numel(), tokens, page, stream_of(lens)),
+                        ip(pos), ip(slots), ip(missing), b, width, pages, tokens, page, stream_of(lens)),
         "tybok_page_plan");
   return {lens2, table2, stack2, count2, cu, pos, slots, missing};
 }
