@@ -6,6 +6,9 @@
 // inside a tile; then it leaves (maximum, sum, unnormalised output) of its part behind, and a second kernel joins the parts in
 // their order.  Queries of the same key head are rows of the same product (row = token * H / G + head).
 //
+// Where the tiles are few and the caches short, a cluster of CTAs takes each tile instead and joins its parts over distributed
+// shared memory: no second kernel, no trip through global memory.
+//
 // Algorithmic bytes: Q and O once, K and V of a request's keys once per row tile (L2 serves the tiles after the first).
 // Flops: 4 * D * H per visible (query, key) pair.
 #include <cuda_bf16.h>
@@ -44,6 +47,7 @@ struct PagedAttnParams {
   int tile_tokens;   // tokens of a tile where it holds whole ones, else 0
   int wide_out;      // the outputs are 32-byte aligned
   int join_blocks;   // what leaving a tile to two CTAs costs, in key blocks
+  int cluster;       // > 0: one row tile per cluster of that many CTAs, which share its key blocks and join their parts themselves
   float scale_log2e;     // softmax scale * log2(e), with its sign
   float abs_scale_log2e; // its magnitude, above zero, and the bit of the scores' instruction that negates Q instead
   uint32_t negate_q;
@@ -87,20 +91,30 @@ __device__ __forceinline__ int pa_tiles(const PagedAttnParams& p, int n) {
   return (n * p.ratio + p.tile_rows - 1) / p.tile_rows;
 }
 
-// ws: int4 per CTA (request, key head, tile, parts of the tile that this CTA begins and others go on with; parts = 0: none), then
-// two partial tiles per CTA: [0] ends a tile begun by another CTA, [1] begins one that others go on with.
+// ws: per CTA what the joining kernel is to know of the tile that it begins and others go on with, then two partial tiles per CTA: [0] ends
+// a tile begun by another CTA, [1] begins one that others go on with.
+struct __align__(16) PaHeader {
+  int parts;        // CTAs that have a part of the tile; 0 = there is none to join
+  int rows, first;  // rows of the tile, and the first one's number among the request's
+  int start, g;     // first token of the request, key head
+  int pad[3];
+};
 template <int ROWS, int D>
 __host__ __device__ constexpr size_t pa_part_bytes() { return static_cast<size_t>(ROWS) * (D + 2) * 4; }
-__host__ __device__ constexpr size_t pa_header_bytes(int ctas) { return (static_cast<size_t>(ctas) * 16 + 255) & ~size_t(255); }
+__host__ __device__ constexpr size_t pa_header_bytes(int ctas) { return (static_cast<size_t>(ctas) * sizeof(PaHeader) + 255) & ~size_t(255); }
 
 // ------------------------------------------------------------------------------------------------ sixteen-row form
 // Few rows per key head (single tokens): 16 rows of mma.m16n8k16, four warps that share the keys of a block and nothing else: each
 // streams its own keys through its own ring and keeps its own maxima, sums and output in registers; they meet at the end of a tile.
 constexpr int PR_ROWS = 16, PR_WARPS = 4, PR_THREADS = 128, PR_STAGES = 3;
-__host__ __device__ constexpr int pr_sub(int d) { return d == 256 ? 16 : 32; }   // keys per warp and block: 16 KB of K and V
-__host__ __device__ constexpr int pr_block(int d) { return PR_WARPS * pr_sub(d); }
-constexpr int PR_STAGE_BYTES = 16384;
-constexpr int PR_SMEM = PR_WARPS * PR_STAGES * PR_STAGE_BYTES;
+constexpr int PR_SUB = 16;                                                            // keys per warp and block
+constexpr int PR_BLOCK = PR_WARPS * PR_SUB;
+__host__ __device__ constexpr int pr_stage(int d) { return 2 * PR_SUB * d * 2; }      // a warp's keys and values of a block
+__host__ __device__ constexpr int pr_ring(int d) { return PR_WARPS * PR_STAGES * pr_stage(d); }
+__host__ __device__ constexpr int pr_smem(int d) { return pr_ring(d) + PR_ROWS * (d + 2) * 4; }  // and what a cluster's CTAs send
+// CTAs per SM.  At head_dim 128 one's copies go on while the other joins its warps' parts or begins a tile; at 256 the ring that keeps
+// memory busy fills the SM.
+__host__ __device__ constexpr int pr_ctas(int d) { return d == 128 ? 2 : 1; }
 
 __device__ __forceinline__ float pa_exp2(float x) {
   float y;
@@ -171,6 +185,7 @@ __device__ __forceinline__ uint32_t pa_scan(uint32_t x) {  // inclusive sums ove
 template <int BK>
 __device__ __forceinline__ uint32_t pa_cost(const PagedAttnParams& p, const PaRequest& r, int tiles) {
   uint32_t cost = 0;
+  if (p.cluster) return tiles;  // (a line of tiles)
   if (!p.causal) return static_cast<uint32_t>(tiles) * max(1, (r.len + BK - 1) / BK);
   const bool many = tiles > 8;  // their sums by the whole warp
   if (!many)
@@ -249,6 +264,12 @@ __device__ __forceinline__ PaPlace pa_locate(const PagedAttnParams& p, const PaL
   at.tiles = __shfl_sync(0xffffffffu, g.tiles, src);
   at.g = p.G == 1 ? 0 : static_cast<int>(x / per_head);
   x -= at.g * per_head;
+  if (p.cluster) {
+    at.tile = static_cast<int>(x);
+    at.blk = 0;
+    at.nblk = pa_blocks<BK>(p, at.r, at.tile);
+    return at;
+  }
   if (!p.causal) {
     at.nblk = max(1, (at.r.len + BK - 1) / BK);
     at.tile = static_cast<int>(x / at.nblk);
@@ -303,6 +324,17 @@ template <int BK>
 __device__ PaShare pa_share(const PagedAttnParams& p, PaPlace& first) {
   const PaLine line = pa_line<BK>(p);
   PaShare sh;
+  if (p.cluster) {  // tile number blockIdx.x / cluster; `per` blocks of it to each CTA
+    sh.whole = false;
+    sh.per = sh.x0 = sh.x1 = 0;
+    const uint32_t x = blockIdx.x / p.cluster, rank = blockIdx.x % p.cluster;
+    if (x >= line.tiles) return sh;
+    first = pa_locate<BK>(p, line, x);
+    sh.per = (first.nblk + p.cluster - 1) / p.cluster;
+    first.blk = min(static_cast<uint32_t>(first.nblk), rank * sh.per);
+    sh.x1 = min(static_cast<uint32_t>(first.nblk) - first.blk, sh.per);
+    return sh;
+  }
   const uint32_t ctas = gridDim.x;
   sh.per = (line.blocks + ctas - 1) / ctas;
   // rounds * average length of a tile against an even share
@@ -325,6 +357,23 @@ __device__ PaShare pa_share(const PagedAttnParams& p, PaPlace& first) {
   first = next;
   return sh;
 }
+__device__ __forceinline__ float4 pa_peer4(const void* local, int rank) {  // 16 bytes of another CTA of the cluster
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(dsmem_addr(smem_u32(local), rank)));
+  return v;
+}
+__device__ __forceinline__ void pa_send4(const void* local, int rank, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dsmem_addr(smem_u32(local), rank)), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ void pa_send(const void* local, int rank, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dsmem_addr(smem_u32(local), rank)), "f"(v) : "memory");
+}
+__device__ __forceinline__ float pa_peer(const void* local, int rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(dsmem_addr(smem_u32(local), rank)));
+  return v;
+}
+
 // How many CTAs the tile has that begins at x in this CTA's share and goes on behind it.
 __device__ __forceinline__ int pa_parts(const PagedAttnParams& p, const PaShare& sh, uint32_t x, int nblk) {
   const uint32_t last = (x + nblk - 1) / sh.per;
@@ -352,90 +401,93 @@ __device__ __forceinline__ void pa_zero_rows(const PagedAttnParams& p, int t, in
 }
 
 template <int D>
-__global__ void __launch_bounds__(PR_THREADS, 1) paged_rows_kernel(const PagedAttnParams p) {
-  extern __shared__ __align__(128) uint8_t pr_smem[];
+__global__ void __launch_bounds__(PR_THREADS, pr_ctas(D)) paged_rows_kernel(const PagedAttnParams p) {
+  extern __shared__ __align__(128) uint8_t pr_shared[];
   __shared__ float s_m[PR_WARPS][PR_ROWS], s_l[PR_WARPS][PR_ROWS];
-  constexpr int SUB = pr_sub(D), BK = pr_block(D), ROW_BYTES = D * 2, CHUNKS = D / 8, KS = D / 16;
+  constexpr int SUB = PR_SUB, BK = PR_BLOCK, STAGE = pr_stage(D), ROW_BYTES = D * 2, CHUNKS = D / 8, KS = D / 16;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (p.cluster) cluster_arrive_relaxed();  // this CTA is there: its shared memory may be written
   if (p.pdl) {
     pdl_launch_dependents();
     pdl_wait();
   }
-  pa_check(p, tid, PR_THREADS);
-  pa_zero_rows<D>(p, tid, PR_THREADS);
   PaPlace at{};
   const PaShare share = pa_share<BK>(p, at);
   const uint32_t x1 = share.x1;
   uint32_t x = share.x0;
-  int4 header = make_int4(0, 0, 0, 0);
-  const uint32_t ring = smem_u32(pr_smem) + warp * (PR_STAGES * PR_STAGE_BYTES);
+  PaHeader header{};
+  // cluster: [CTA][row of this CTA's share][D], then the references and the sums, as the CTAs send them
+  float* parts = reinterpret_cast<float*>(pr_shared + pr_ring(D));
+  const int each = p.cluster ? PR_ROWS / p.cluster : PR_ROWS, rank = p.cluster ? static_cast<int>(cluster_ctarank()) : 0;
+  bool tidied = false;
+  auto tidy = [&] {  // under the first keys' way
+    pa_check(p, tid, PR_THREADS);
+    pa_zero_rows<D>(p, tid, PR_THREADS);
+    tidied = true;
+  };
+  const uint32_t ring = smem_u32(pr_shared) + warp * (PR_STAGES * STAGE);
   while (x < x1) {
     const int end = static_cast<int>(min(static_cast<uint32_t>(at.nblk), at.blk + (x1 - x)));
     const int rows = at.r.n * p.ratio;
-    // this thread's two rows of the tile: queries as operand fragments, keys they see
-    uint32_t qf[KS][4];
-    int limit[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = at.tile * PR_ROWS + h * 8 + (lane >> 2), token = row / p.ratio;
-      const bool live = row < rows;
-      limit[h] = !live ? 0 : p.causal ? max(0, at.r.len - at.r.n + token + 1) : at.r.len;
-      const __nv_bfloat16* src = p.q + (at.r.start + token) * p.ldq + static_cast<long long>(at.g * p.ratio + row - token * p.ratio) * D + (lane & 3) * 2;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        qf[ks][h] = live ? *reinterpret_cast<const uint32_t*>(src + ks * 16) : 0u;
-        qf[ks][h + 2] = live ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8) : 0u;
-      }
-    }
     const int seen = pa_seen(p, at.r, min(rows, (at.tile + 1) * PR_ROWS));                    // by any row
     const int seen_all = p.causal ? max(0, at.r.len - at.r.n + at.tile * PR_ROWS / p.ratio + 1) : at.r.len;  // by every row
+    uint32_t in = 0, out = 0;  // ring slots
     auto fetch = [&](int j) {  // this warp's keys of block j
-      const uint32_t slot = ring + (j % PR_STAGES) * PR_STAGE_BYTES;
-      const int key0 = j * BK + warp * SUB;
-#pragma unroll 1
-      for (int k0 = 0; k0 < SUB; k0 += 16) {
-        const int key = key0 + k0;
-        int page = -1;
-        if (key < seen) {
-          page = p.table[at.b * p.ld_table + (key >> p.page_shift)];
-          if (page < 0 || page >= p.P) {
-            if (p.status && lane == 0) atomicCAS(p.status, 0, TYBOK_DEV_BAD_INDEX);
-            page = -1;
-          }
-        }
-        const long long off = key & ((1 << p.page_shift) - 1), pg = max(page, 0);
-        const __nv_bfloat16* ks = p.kp + pg * p.k_page + at.g * p.k_head + off * p.k_row;
-        const __nv_bfloat16* vs = p.vp + pg * p.v_page + at.g * p.v_head + off * p.v_row;
-#pragma unroll
-        for (int i = 0; i < 16 * CHUNKS / 32; ++i) {
-          const int r = (i * 32 + lane) / CHUNKS, c = (i * 32 + lane) % CHUNKS;
-          const int bytes = page >= 0 && key + r < seen ? 16 : 0;  // the others are zero
-          const uint32_t dst = slot + (k0 + r) * ROW_BYTES + ((c ^ (r & 7)) << 4);
-          const long long rr = bytes ? r : 0;
-          cp_async16(dst, ks + rr * p.k_row + c * 8, bytes);
-          cp_async16(dst + SUB * ROW_BYTES, vs + rr * p.v_row + c * 8, bytes);
+      const uint32_t slot = ring + in * STAGE;
+      in = in + 1 == PR_STAGES ? 0 : in + 1;
+      const int key = j * BK + warp * SUB;  // sixteen keys lie in one page
+      int page = -1;
+      if (key < seen) {
+        page = p.table[at.b * p.ld_table + (key >> p.page_shift)];
+        if (page < 0 || page >= p.P) {
+          if (p.status && lane == 0) atomicCAS(p.status, 0, TYBOK_DEV_BAD_INDEX);
+          page = -1;
         }
       }
+      const long long off = key & ((1 << p.page_shift) - 1), pg = max(page, 0);
+      const __nv_bfloat16* ks = p.kp + pg * p.k_page + at.g * p.k_head + off * p.k_row;
+      const __nv_bfloat16* vs = p.vp + pg * p.v_page + at.g * p.v_head + off * p.v_row;
+#pragma unroll
+      for (int i = 0; i < SUB * CHUNKS / 32; ++i) {
+        const int r = (i * 32 + lane) / CHUNKS, c = (i * 32 + lane) % CHUNKS;
+        const int bytes = page >= 0 && key + r < seen ? 16 : 0;  // the others are zero
+        const uint32_t dst = slot + r * ROW_BYTES + ((c ^ (r & 7)) << 4);
+        const long long rr = bytes ? r : 0;
+        cp_async16(dst, ks + rr * p.k_row + c * 8, bytes);
+        cp_async16(dst + SUB * ROW_BYTES, vs + rr * p.v_row + c * 8, bytes);
+      }
     };
+    uint32_t qf[KS][4];
+    int limit[2];
+        // this thread's two rows of the tile: queries as operand fragments, keys they see
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = at.tile * PR_ROWS + h * 8 + (lane >> 2), token = row / p.ratio;
+          const bool live = row < rows;
+          limit[h] = !live ? 0 : p.causal ? max(0, at.r.len - at.r.n + token + 1) : at.r.len;
+          const __nv_bfloat16* src = p.q + (at.r.start + token) * p.ldq + static_cast<long long>(at.g * p.ratio + row - token * p.ratio) * D + (lane & 3) * 2;
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            qf[ks][h] = live ? *reinterpret_cast<const uint32_t*>(src + ks * 16) : 0u;
+            qf[ks][h + 2] = live ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8) : 0u;
+          }
+        }
     float o[D / 8][4];
 #pragma unroll
     for (int i = 0; i < D / 8; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < PR_STAGES - 1; ++i) {
-      if (at.blk + i < end) fetch(at.blk + i);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
 #pragma unroll 1
-    for (int j = at.blk; j < end; ++j) {
+    for (int j = at.blk - (PR_STAGES - 1); j < end; ++j) {  // (the code that fetches once)
       if (j + PR_STAGES - 1 < end) fetch(j + PR_STAGES - 1);
       asm volatile("cp.async.commit_group;" ::: "memory");
+      if (j < at.blk) continue;
+      if (j == at.blk && !tidied) tidy();
       asm volatile("cp.async.wait_group %0;" ::"n"(PR_STAGES - 1) : "memory");
       __syncwarp();
       const int key0 = j * BK + warp * SUB;
-      const uint32_t ka = ring + (j % PR_STAGES) * PR_STAGE_BYTES, va = ka + SUB * ROW_BYTES;
+      const uint32_t ka = ring + out * STAGE, va = ka + SUB * ROW_BYTES;
       if (key0 < seen) {
         float sc[SUB / 8][4];
 #pragma unroll
@@ -502,12 +554,13 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_rows_kernel(const PagedAt
           }
         }
       }
+      out = out + 1 == PR_STAGES ? 0 : out + 1;
       __syncwarp();
     }
     // the four warps' parts meet
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncwarp();
-    float* mine = reinterpret_cast<float*>(pr_smem + warp * (PR_STAGES * PR_STAGE_BYTES));
+    float* mine = reinterpret_cast<float*>(pr_shared + warp * (PR_STAGES * STAGE));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -522,24 +575,24 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_rows_kernel(const PagedAt
         *reinterpret_cast<float2*>(mine + row * D + ((i * 8 + (lane & 3) * 2) ^ ((row & 3) << 3))) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
     }
     __syncthreads();
-    const bool whole_tile = at.blk == 0 && end == at.nblk;
+    const bool whole_tile = !p.cluster && at.blk == 0 && end == at.nblk;
     const int part = at.blk > 0 ? 0 : 1;
+    if (p.cluster) cluster_wait_acquire();  // the others are there
     float* po = reinterpret_cast<float*>(p.ws + pa_header_bytes(gridDim.x) + (2ll * blockIdx.x + part) * pa_part_bytes<PR_ROWS, D>());
-#pragma unroll 1
+#pragma unroll
     for (int i = tid; i < PR_ROWS * D / 8; i += PR_THREADS) {
       const int row = i / (D / 8), c = (i % (D / 8)) * 8;
-      float top = -INFINITY;
+      float f[PR_WARPS], top = -INFINITY, sum = 0.f, v[8] = {};
 #pragma unroll
       for (int w = 0; w < PR_WARPS; ++w) top = fmaxf(top, s_m[w][row]);
-      float sum = 0.f, v[8] = {};
 #pragma unroll
       for (int w = 0; w < PR_WARPS; ++w) {
-        const float f = pa_exp2(s_m[w][row] - (top == -INFINITY ? 0.f : top));
-        sum += f * s_l[w][row];
-        const float4* src = reinterpret_cast<const float4*>(pr_smem + w * (PR_STAGES * PR_STAGE_BYTES)) + (row * D + (c ^ ((row & 3) << 3))) / 4;
+        f[w] = pa_exp2(s_m[w][row] - (top == -INFINITY ? 0.f : top));
+        sum += f[w] * s_l[w][row];
+        const float4* src = reinterpret_cast<const float4*>(pr_shared + w * (PR_STAGES * STAGE)) + (row * D + (c ^ ((row & 3) << 3))) / 4;
         const float4 a = src[0], b = src[1];
-        v[0] += f * a.x; v[1] += f * a.y; v[2] += f * a.z; v[3] += f * a.w;
-        v[4] += f * b.x; v[5] += f * b.y; v[6] += f * b.z; v[7] += f * b.w;
+        v[0] += f[w] * a.x; v[1] += f[w] * a.y; v[2] += f[w] * a.z; v[3] += f[w] * a.w;
+        v[4] += f[w] * b.x; v[5] += f[w] * b.y; v[6] += f[w] * b.z; v[7] += f[w] * b.w;
       }
       const int grow = at.tile * PR_ROWS + row;
       if (grow >= rows) continue;
@@ -549,6 +602,14 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_rows_kernel(const PagedAt
         for (int e = 0; e < 8; ++e) v[e] *= inv;
         const int token = grow / p.ratio;
         pa_store8(p, (at.r.start + token) * p.ld_out + static_cast<long long>(at.g * p.ratio + grow - token * p.ratio) * D + c, v);
+      } else if (p.cluster) {
+        const int owner = row / each, at_owner = rank * each + row % each;
+        pa_send4(parts + at_owner * D + c, owner, make_float4(v[0], v[1], v[2], v[3]));
+        pa_send4(parts + at_owner * D + c + 4, owner, make_float4(v[4], v[5], v[6], v[7]));
+        if (c == 0) {
+          pa_send(parts + PR_ROWS * D + at_owner, owner, top);
+          pa_send(parts + PR_ROWS * D + PR_ROWS + at_owner, owner, sum);
+        }
       } else {
         float4* dst = reinterpret_cast<float4*>(po + row * D + c);
         dst[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -559,12 +620,51 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_rows_kernel(const PagedAt
         }
       }
     }
-    if (!whole_tile && at.blk == 0) header = make_int4(at.b, at.g, at.tile, pa_parts(p, share, x, at.nblk));
+    if (p.cluster) break;
+    if (!whole_tile && at.blk == 0) header = {pa_parts(p, share, x, at.nblk), min(PR_ROWS, rows - at.tile * PR_ROWS), at.tile * PR_ROWS, at.r.start, at.g};
     x += end - at.blk;
     __syncthreads();  // the ring is free again
     if (x < x1) pa_next<BK>(p, at);
   }
-  if (tid == 0) reinterpret_cast<int4*>(p.ws)[blockIdx.x] = header;
+  if (!tidied) tidy();
+  if (!p.cluster) {
+    if (tid == 0) reinterpret_cast<PaHeader*>(p.ws)[blockIdx.x] = header;
+    return;
+  }
+  if (x == x1) {  // a CTA without blocks has nothing to add
+    cluster_wait_acquire();
+    if (share.per > 0 && tid < PR_ROWS) pa_send(parts + PR_ROWS * D + rank * each + tid % each, tid / each, -INFINITY);
+  }
+  __syncwarp();
+  cluster_sync_all();  // every part has arrived
+  if (share.per == 0) return;  // no tile for the whole cluster
+  const int rows = at.r.n * p.ratio;
+  for (int i = tid; i < each * D / 8; i += PR_THREADS) {
+    const int mine = i / (D / 8), c = (i % (D / 8)) * 8, row = rank * each + mine, grow = at.tile * PR_ROWS + row;
+    if (grow >= rows) continue;
+    float m[8], top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      m[k] = k < p.cluster ? parts[PR_ROWS * D + k * each + mine] : -INFINITY;
+      top = fmaxf(top, m[k]);
+    }
+    float sum = 0.f, v[8] = {};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (m[k] == -INFINITY) continue;
+      const float f = pa_exp2(m[k] - top);
+      sum += f * parts[PR_ROWS * D + PR_ROWS + k * each + mine];
+      const float4* src = reinterpret_cast<const float4*>(parts + (k * each + mine) * D + c);
+      const float4 a = src[0], b = src[1];
+      v[0] += f * a.x; v[1] += f * a.y; v[2] += f * a.z; v[3] += f * a.w;
+      v[4] += f * b.x; v[5] += f * b.y; v[6] += f * b.z; v[7] += f * b.w;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= inv;
+    const int token = grow / p.ratio;
+    pa_store8(p, (at.r.start + token) * p.ld_out + static_cast<long long>(at.g * p.ratio + grow - token * p.ratio) * D + c, v);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ tile forms
@@ -647,6 +747,8 @@ struct __align__(16) PtBars {
   volatile int abort;
   float m_ref[2][128];                       // wide: per group and row
   float end_m[2][2][128], end_l[2][2][128];  // wide: per parity of the tile, group and row
+  PtPiece item;                              // cluster: the tile (rows = 0: none), and this CTA's part of its statistics
+  float part_m[256], part_l[256];
 };
 
 // Piece n, read by a whole warp; false when there is none or the CTA has given up.
@@ -679,26 +781,74 @@ __device__ __forceinline__ bool pt_wait(const PtWait& a, const PtWait& b, const 
   return __all_sync(0xffffffffu, wait_or_abort(which == 0 ? a.bar : which == 1 ? b.bar : c.bar, which == 0 ? a.parity : which == 1 ? b.parity : c.parity, abort_flag));
 }
 
+// How many of a block's weights (32 keys at a time) after the first have been handed over, in their order.
+template <int N>
+__device__ __forceinline__ int pt_handed(uint64_t* handed, uint32_t parity) {
+  const int lane = threadIdx.x & 31;
+  return __ffs(~__ballot_sync(0xffffffffu, lane < N - 1 && mbar_test_wait(&handed[1 + min(lane, N - 2)], parity))) - 1;
+}
+
+// What an issuing warp is about to need: a block's weights, 32 keys at a time (parts), its values, and the keys of the scores after it.  A wait
+// is a round trip of a hundred clocks even where the phase has passed, and the tensor core runs dry meanwhile (it holds a
+// few instructions).  So lanes ask for different barriers at once, and for a turn while the one before is still being issued.
+struct PtTurn {
+  uint64_t *parts, *values, *keys;
+  uint32_t part_parity, value_parity, key_parity;
+  bool more;  // the keys count
+  // The barrier that this lane asks for.
+  template <int N>
+  __device__ __forceinline__ bool lane_done(int lane) const {
+    uint64_t* bar = lane < N ? parts + lane : lane == N ? values : keys;
+    const uint32_t parity = lane < N ? part_parity : lane == N ? value_parity : key_parity;
+    return lane > N + 1 || (lane == N + 1 && !more) || mbar_test_wait(bar, parity & 1);
+  }
+  // Parts that need no wait: none unless the values and keys are there.
+  template <int N>
+  __device__ __forceinline__ int ready() const {
+    const uint32_t done = __ballot_sync(0xffffffffu, lane_done<N>(threadIdx.x & 31));
+    return ((done >> N) & 3u) == 3u ? __ffs(~(done & ((1u << N) - 1u))) - 1 : 0;
+  }
+  // Until the values, the keys and one part are there; 0 when the CTA has given up.
+  template <int N>
+  __device__ __forceinline__ int wait(volatile int* abort_flag) const {
+    int n = ready<N>();
+    const long long t0 = clock64();
+    while (n == 0) {
+      if (*abort_flag || clock64() - t0 > kWaitLimitCycles) break;
+      n = ready<N>();
+    }
+    return __shfl_sync(0xffffffffu, n, 0);
+  }
+};
+
 // Products whose descriptors differ in the low word only (start address, leading offset): the high word (stride 1024 bytes, version,
 // 128-byte swizzle) is a constant.
 constexpr uint32_t PT_DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
 __device__ __forceinline__ uint32_t pt_desc_lo(uint32_t smem_addr, uint32_t chunk_bytes) { return (smem_addr & 0x3FFFF) >> 4 | chunk_bytes >> 4 << 16; }
-__device__ __forceinline__ void pt_mma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+// By the lane with `leader` set; predicated, so that the warp's control flow stays uniform.
+__device__ __forceinline__ void pt_mma_ss(uint32_t leader, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
       "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(PT_DESC_HI)
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(PT_DESC_HI), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void pt_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void pt_mma_ts(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
       "mov.b64 b, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(PT_DESC_HI)
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(PT_DESC_HI), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void pt_commit(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+      "r"(leader)
       : "memory");
 }
 
@@ -712,7 +862,16 @@ template <int D>
 __device__ __forceinline__ void pt_lead(const PagedAttnParams& p, PaPlace at, const PaShare& share, const CUtensorMap* map, uint8_t* sq, PtBars& bars) {
   constexpr int NCH = D / 64, CH = 16384, TILES = pt_rows(D) / 128;
   const int lane = threadIdx.x & 31, tokens = p.tile_tokens / TILES, half = tokens * p.ratio;
-  int4 header = make_int4(0, 0, 0, 0);
+  PaHeader header{};
+  if (p.cluster && lane == 0) {
+    PtPiece w{};
+    if (share.per > 0) {
+      w.rows = min(p.tile_rows, at.r.n * p.ratio - at.tile * p.tile_rows);
+      w.g = at.g;
+      w.token = at.r.start + at.tile * p.tile_tokens;
+    }
+    bars.item = w;
+  }
   uint32_t n = 0, queries = 0;
   bool ok = true;
   uint32_t x = share.x0;
@@ -733,8 +892,8 @@ __device__ __forceinline__ void pt_lead(const PagedAttnParams& p, PaPlace at, co
       w.seen = p.causal ? at.r.len - at.r.n + first + 1 : at.r.len;
       w.step = p.causal;
       w.token = at.r.start + first;
-      w.part = w.blk == 0 && w.end == at.nblk ? 0 : w.blk > 0 ? 1 : 2;
-      if (w.part == 2) header = make_int4(at.b, at.g, at.tile, pa_parts(p, share, x, at.nblk));
+      w.part = p.cluster ? 1 : w.blk == 0 && w.end == at.nblk ? 0 : w.blk > 0 ? 1 : 2;
+      if (w.part == 2) header = {pa_parts(p, share, x, at.nblk), w.rows, at.tile * p.tile_rows, at.r.start, at.g};
     }
     if (lane == 0) {
       bars.piece[s] = w;
@@ -756,7 +915,7 @@ __device__ __forceinline__ void pt_lead(const PagedAttnParams& p, PaPlace at, co
     if (x < share.x1) pa_next<pt_bk(D)>(p, at);
   }
   if (queries > 0) mbar_wait(&bars.q_full, (queries - 1) & 1);
-  if (lane == 0) reinterpret_cast<int4*>(p.ws)[blockIdx.x] = header;
+  if (lane == 0 && !p.cluster) reinterpret_cast<PaHeader*>(p.ws)[blockIdx.x] = header;
 }
 
 // Keys (values) of the share: one block after the other into a ring of two.  A block's boxes: lane = piece of the block * chunks + chunk of
@@ -873,23 +1032,24 @@ __device__ __forceinline__ void pt_part32(float4* part, int column, int row, con
     part[(column / 4 + e) * 128 + row] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
 }
 
-// Masks, maximum, exponentials and the bf16 weights of N words of 32 scores of one row; `seen` keys of them count.
+// Masks, maximum, exponentials and the bf16 weights of 32 scores of one row, of which the first `left` keys count.
 template <int N>
-__device__ __forceinline__ float pt_row_max(uint32_t (&v)[N][32], int seen) {
-  float mx[4] = {-1e30f, -1e30f, -1e30f, -1e30f};
+__device__ __forceinline__ void pt_row_max(uint32_t (&v)[32], int left, float (&mx)[N]) {
+  if (left < 32) {
+    const uint32_t bits = left <= 0 ? 0u : (1u << left) - 1u;
 #pragma unroll
-  for (int w = 0; w < N; ++w) {
-    if (seen < 32 * N) {
-      const int left = seen - 32 * w;
-      const uint32_t bits = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
-#pragma unroll
-      for (int e = 0; e < 32; ++e)
-        if (!((bits >> e) & 1u)) v[w][e] = PA_MASKED;
-    }
-#pragma unroll
-    for (int e = 0; e < 32; e += 2) mx[w & 3] = pt_max3(mx[w & 3], __uint_as_float(v[w][e]), __uint_as_float(v[w][e + 1]));
+    for (int e = 0; e < 32; ++e)
+      if (!((bits >> e) & 1u)) v[e] = PA_MASKED;
   }
-  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+#pragma unroll
+  for (int e = 0; e < 32; e += 2) mx[(e >> 1) % N] = pt_max3(mx[(e >> 1) % N], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+}
+// Ties 32 registers to this point of the program: their load has been waited for.
+__device__ __forceinline__ void pt_landed(uint32_t (&v)[32]) {
+  asm volatile("" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
+               "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]),
+               "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]));
+  asm volatile("" : "+r"(v[30]), "+r"(v[31]));
 }
 __device__ __forceinline__ void pt_weights(const uint32_t (&v)[32], uint64_t c2, uint64_t nm, uint64_t& sum, uint32_t (&pk)[16]) {
 #pragma unroll
@@ -955,6 +1115,7 @@ __device__ __forceinline__ PaShare pt_begin(const PagedAttnParams& p, PtBars& ba
     bars.abort = 0;
     fence_barrier_init();
   }
+  if (p.cluster && tid >= 128) bars.part_m[tid - 128] = -INFINITY;
   if (warp == 1) {
     tmem_alloc(&bars.tmem_base, 512);
     tmem_relinquish();
@@ -973,10 +1134,16 @@ __device__ __forceinline__ PaShare pt_begin(const PagedAttnParams& p, PtBars& ba
 template <int N>
 __device__ __forceinline__ float pt_scores(uint32_t t_s, uint32_t (&v)[N][32], int seen, float scale) {
   tc_fence_after();
+  float mx[4] = {-1e30f, -1e30f, -1e30f, -1e30f};
+  tmem_ld32(t_s, v[0]);
 #pragma unroll
-  for (int w = 0; w < N; ++w) tmem_ld32(t_s + w * 32, v[w]);
-  tc_wait_ld();
-  return pt_row_max<N>(v, seen) * scale;
+  for (int w = 0; w < N; ++w) {  // 32 scores' maximum under the load of the next ones
+    tc_wait_ld();
+    pt_landed(v[w]);
+    if (w + 1 < N) tmem_ld32(t_s + (w + 1) * 32, v[w + 1 < N ? w + 1 : 0]);
+    pt_row_max<4>(v[w], seen - 32 * w, mx);
+  }
+  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
 }
 // ... and the weights relative to m over them, handed over 32 keys at a time (the last ones by the caller); returns their sum.
 template <int N>
@@ -1011,6 +1178,50 @@ __device__ __forceinline__ void pt_hand_over(bool live, uint64_t* handed) {
   }
 }
 
+// The CTAs of a cluster join their parts of a tile, each for its share of the rows: a thread per row and 32 columns, parts in their order.
+// All of the CTA's work on its own part is done and visible to its threads.
+template <int D>
+__device__ __forceinline__ void pt_join(const PagedAttnParams& p, PtBars& bars, const float4* part) {
+  if (bars.item.rows == 0) return;  // no tile for the whole cluster
+  cluster_sync_all();
+  if (threadIdx.x >= 128) {  // (the warps with registers)
+    const int each = pt_rows(D) / p.cluster, rank = cluster_ctarank(), half = p.tile_rows / (pt_rows(D) / 128);
+    for (int i = threadIdx.x - 128; i < each * (D / 32); i += 256) {
+      const int at = rank * each + i % each, c = i / each, t = at >> 7, local = t * half + (at & 127);
+      if ((at & 127) >= half || local >= bars.item.rows) continue;
+      float m[8], l[8], top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        m[k] = k < p.cluster ? pa_peer(&bars.part_m[at], k) : -INFINITY;  // (of a CTA without blocks, too)
+        l[k] = k < p.cluster ? pa_peer(&bars.part_l[at], k) : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, m[k]);
+      uint32_t o[32] = {};
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (m[k] == -INFINITY) continue;
+        const float f = pa_exp2(m[k] - top);
+        sum += f * l[k];
+        const float4* src = part + (t * (D / 4) + c * 8) * 128 + (at & 127);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float4 a = pa_peer4(src + e * 128, k);
+          o[4 * e] = __float_as_uint(__uint_as_float(o[4 * e]) + f * a.x);
+          o[4 * e + 1] = __float_as_uint(__uint_as_float(o[4 * e + 1]) + f * a.y);
+          o[4 * e + 2] = __float_as_uint(__uint_as_float(o[4 * e + 2]) + f * a.z);
+          o[4 * e + 3] = __float_as_uint(__uint_as_float(o[4 * e + 3]) + f * a.w);
+        }
+      }
+      const int ahead = local / p.ratio;
+      pt_store32(p, static_cast<long long>(bars.item.token + ahead) * p.ld_out + static_cast<long long>(bars.item.g * p.ratio + local - ahead * p.ratio) * D + c * 32, o,
+                 sum == 0.f ? 0.f : 1.f / sum);
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();  // nobody's part is read any more
+}
+
 __global__ void __launch_bounds__(PT_THREADS, 1)
 paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                   const PagedAttnParams p) {
@@ -1034,7 +1245,7 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const PtRing rings[1] = {{k ? &tm_k : &tm_v, k ? sk : sv, k ? bars.k_full : bars.v_full, k ? bars.k_empty : bars.v_empty}};
       pt_stream<D, 1>(p, rings, bars);
     } else {
-      const bool leader = elect_one();
+      const uint32_t leader = elect_one();
       const uint32_t idesc_s = idesc_bf16_f32(128, BK) | p.negate_q, idesc_o = idesc_bf16_f32(128, D) | (1u << 16);
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -1064,15 +1275,15 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
               if (!ok) break;
               tc_fence_after();
               if (t == 0) pt_clear_tail<D>(sv + (vb & 1) * KV, len, blk + j);
+              int ready = 0;  // parts after the first that need no wait
 #pragma unroll
               for (int part = 0; part < 4; ++part) {  // each 32 keys' product starts under the next ones' exponentials
-                if (part) {
-                  if (!wait(&bars.p_full[t][part], weights.parity)) break;
-                  tc_fence_after();
-                }
+                if (part == 1) ready = pt_handed<4>(bars.p_full[t], weights.parity);
+                if (part > ready && !wait(&bars.p_full[t][part], weights.parity)) break;
+                if (part) tc_fence_after();
 #pragma unroll
                 for (int ks = 2 * part; ks < 2 * part + 2; ++ks)
-                  if (leader) pt_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, v_desc + ks * (2048 >> 4), idesc_o, j > 0 || ks ? 1u : 0u);
+                  pt_mma_ts(leader, tmem + 256 + t * 128, tmem + t * 128 + ks * 8, v_desc + ks * (2048 >> 4), idesc_o, j > 0 || ks ? 1u : 0u);
               }
             }
             if (!ok) break;
@@ -1081,27 +1292,24 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll
               for (int ks = 0; ks < 8; ++ks) {
                 const uint32_t o = (ks >> 2) * (CH >> 4) + (ks & 3) * 2;
-                if (leader) pt_mma_ss(tmem + t * 128, q_desc + o, k_desc + o, idesc_s, ks > 0 ? 1u : 0u);
+                pt_mma_ss(leader, tmem + t * 128, q_desc + o, k_desc + o, idesc_s, ks > 0 ? 1u : 0u);
               }
-              if (leader) tc_commit(&bars.s_full[t]);
-            } else if (leader) {
-              tc_commit(&bars.done[t]);
+              pt_commit(leader, &bars.s_full[t]);
+            } else {
+              pt_commit(leader, &bars.done[t]);
             }
           }
-          if (ok && leader) {
-            if (more) tc_commit(&bars.k_empty[kb & 1]);
-            if (j + 2 == nb) tc_commit(&bars.q_empty);  // the last scores have been issued
-            if (j >= 0) tc_commit(&bars.v_empty[vb & 1]);
-          }
-          __syncwarp();
+          if (!ok) break;
+          if (more) pt_commit(leader, &bars.k_empty[kb & 1]);
+          if (j + 2 == nb) pt_commit(leader, &bars.q_empty);  // the last scores have been issued
+          if (j >= 0) pt_commit(leader, &bars.v_empty[vb & 1]);
         }
         i += nb;
         if (nt == 2) i_second += nb;
       }
       ok = ok && reader.ok;
       // nothing of this CTA's tensor work may be in flight when it gives up its tensor memory
-      if (leader) tc_commit(&bars.mma_done);
-      __syncwarp();
+      pt_commit(leader, &bars.mma_done);
       if (!ok && lane == 0) {
         bars.abort = 1;
         if (p.status) atomicCAS(p.status, 0, TYBOK_DEV_TIMEOUT_MMA);
@@ -1153,7 +1361,7 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         tc_fence_after();
         const float inv = at.part ? 1.f : l == 0.f ? 0.f : 1.f / l;
         // [tile][column / 4][row], then the references and sums of both tiles
-        float4* part = reinterpret_cast<float4*>(p.ws + pa_header_bytes(gridDim.x) + (2ll * blockIdx.x + at.part - 1) * pa_part_bytes<pt_rows(D), D>());
+        float4* part = p.cluster ? reinterpret_cast<float4*>(sk) : reinterpret_cast<float4*>(p.ws + pa_header_bytes(gridDim.x) + (2ll * blockIdx.x + at.part - 1) * pa_part_bytes<pt_rows(D), D>());
         const long long to = static_cast<long long>(at.token + ahead) * p.ld_out + static_cast<long long>(at.g * p.ratio + local - ahead * p.ratio) * D;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
@@ -1165,8 +1373,8 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         }
         if (at.part) {
           float* stat = reinterpret_cast<float*>(part + pt_rows(D) * D / 4);
-          stat[t * 128 + row] = m_ref;
-          stat[pt_rows(D) + t * 128 + row] = l;
+          (p.cluster ? bars.part_m : stat)[t * 128 + row] = m_ref;
+          (p.cluster ? bars.part_l : stat + pt_rows(D))[t * 128 + row] = l;
         }
         tc_fence_before();
       }
@@ -1183,6 +1391,7 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (p.cluster) pt_join<D>(p, bars, reinterpret_cast<const float4*>(sk));
 }
 
 __global__ void __launch_bounds__(PT_THREADS, 1)
@@ -1207,7 +1416,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const PtRing rings[1] = {{k ? &tm_k : &tm_v, k ? sk : sv, k ? bars.k_full : bars.v_full, k ? bars.k_empty : bars.v_empty}};
       pt_stream<D, 1>(p, rings, bars);
     } else {
-      const bool leader = elect_one();
+      const uint32_t leader = elect_one();
       const uint32_t idesc_s = idesc_bf16_f32(128, BK) | p.negate_q, idesc_o = idesc_bf16_f32(128, D) | (1u << 16);
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -1221,13 +1430,22 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const uint32_t n = reader.n - 1;
         const int nb = pt_uniform(at.end - at.blk), blk = pt_uniform(at.blk), len = pt_uniform(at.len);
         if (!wait(&bars.q_in, n & 1)) break;
+        auto turn = [&](int j) {  // product of block j of the piece, then scores of block j + 2
+          const uint32_t vb = i + j, s = vb & 1;
+          return PtTurn{bars.p_full[s], &bars.v_full[s], &bars.k_full[s], vb >> 1, vb >> 1, (vb + 2) >> 1, j + 2 < nb};
+        };
+        int parts = 0;  // of this turn's weights, known to be there
 #pragma unroll 1
         for (int j = -2; j < nb; ++j) {
           const bool more = j + 2 < nb;
-          const uint32_t vb = i + j, kb = i + j + 2, s = vb & 1;  // blocks of this product and of the scores after it, their buffer
-          const PtWait keys{&bars.k_full[s], (kb >> 1) & 1}, values{&bars.v_full[s], (vb >> 1) & 1};
+          const uint32_t vb = i + j, kb = vb + 2, s = vb & 1;  // blocks of this product and of the scores after it, their buffer
           if (j == 0 && n > 0 && !wait(&bars.o_free, (n - 1) & 1)) break;  // the last tile's output has been read
-          ok = j < 0 ? !more || wait(keys.bar, keys.parity) : pt_wait(values, {&bars.p_full[s][0], (vb >> 1) & 1}, more ? keys : values, &bars.abort);
+          if (j >= 0) {
+            if (parts == 0) parts = turn(j).wait<2>(&bars.abort);
+            ok = parts > 0;
+          } else if (more) {
+            wait(&bars.k_full[s], (kb >> 1) & 1);
+          }
           if (!ok) break;
           tc_fence_after();
           if (j >= 0) {
@@ -1235,42 +1453,37 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             const uint32_t v_desc = pt_desc_lo(smem_u32(sv + s * KV), CH);
 #pragma unroll
             for (int part = 0; part < 2; ++part) {  // the first 32 keys' product starts under the others' exponentials
-              if (part) {
+              if (part >= parts) {
                 if (!wait(&bars.p_full[s][1], (vb >> 1) & 1)) break;
                 tc_fence_after();
               }
 #pragma unroll
               for (int ks = 2 * part; ks < 2 * part + 2; ++ks)
-                if (leader) pt_mma_ts(tmem + 256, tmem + s * 64 + ks * 8, v_desc + ks * (2048 >> 4), idesc_o, j > 0 || ks ? 1u : 0u);
+                pt_mma_ts(leader, tmem + 256, tmem + s * 64 + ks * 8, v_desc + ks * (2048 >> 4), idesc_o, j > 0 || ks ? 1u : 0u);
             }
             if (!ok) break;
           }
+          parts = j + 1 >= 0 && j + 1 < nb ? turn(j + 1).ready<2>() : 0;
           if (more) {
             const uint32_t k_desc = pt_desc_lo(smem_u32(sk + s * KV), 16);
 #pragma unroll
             for (int ks = 0; ks < 16; ++ks) {
               const uint32_t o = (ks >> 2) * (CH >> 4) + (ks & 3) * 2;
-              if (leader) pt_mma_ts(tmem + s * 64, tmem + 128 + ks * 8, k_desc + o, idesc_s, ks > 0 ? 1u : 0u);
+              pt_mma_ts(leader, tmem + s * 64, tmem + 128 + ks * 8, k_desc + o, idesc_s, ks > 0 ? 1u : 0u);
             }
+            pt_commit(leader, &bars.s_full[s]);
+            pt_commit(leader, &bars.k_empty[s]);
+            if (j + 3 == nb) pt_commit(leader, &bars.q_used);  // the last scores have been issued
           }
-          if (leader) {
-            if (more) {
-              tc_commit(&bars.s_full[s]);
-              tc_commit(&bars.k_empty[s]);
-              if (j + 3 == nb) tc_commit(&bars.q_used);  // the last scores have been issued
-            }
-            if (j >= 0) {
-              tc_commit(&bars.done[vb & 3]);
-              tc_commit(&bars.v_empty[s]);
-            }
+          if (j >= 0) {
+            pt_commit(leader, &bars.done[vb & 3]);
+            pt_commit(leader, &bars.v_empty[s]);
           }
-          __syncwarp();
         }
         i += nb;
       }
       ok = ok && reader.ok;
-      if (leader) tc_commit(&bars.mma_done);
-      __syncwarp();
+      pt_commit(leader, &bars.mma_done);
       if (!ok && lane == 0) {
         bars.abort = 1;
         if (p.status) atomicCAS(p.status, 0, TYBOK_DEV_TIMEOUT_MMA);
@@ -1374,7 +1587,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       if (live) {
         tc_fence_after();
         const float inv = at.part ? 1.f : l == 0.f ? 0.f : 1.f / l;
-        float4* part = reinterpret_cast<float4*>(p.ws + pa_header_bytes(gridDim.x) + (2ll * blockIdx.x + at.part - 1) * pa_part_bytes<pt_rows(D), D>());
+        float4* part = p.cluster ? reinterpret_cast<float4*>(sk) : reinterpret_cast<float4*>(p.ws + pa_header_bytes(gridDim.x) + (2ll * blockIdx.x + at.part - 1) * pa_part_bytes<pt_rows(D), D>());
         const long long to = static_cast<long long>(at.token + ahead) * p.ld_out + static_cast<long long>(at.g * p.ratio + row - ahead * p.ratio) * D;
 #pragma unroll 1
         for (int c = 4 * grp; c < 4 * grp + 4; ++c) {
@@ -1386,8 +1599,8 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         }
         if (at.part && grp == 0) {
           float* stat = reinterpret_cast<float*>(part + pt_rows(D) * D / 4);
-          stat[row] = m_end;
-          stat[pt_rows(D) + row] = l;
+          (p.cluster ? bars.part_m : stat)[row] = m_end;
+          (p.cluster ? bars.part_l : stat + pt_rows(D))[row] = l;
         }
       }
       tc_fence_before();
@@ -1407,6 +1620,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (p.cluster) pt_join<D>(p, bars, reinterpret_cast<const float4*>(sk));
 }
 
 // Joins the parts of the tile that CTA blockIdx.x of a tile form began: a thread per row and 32 columns.
@@ -1416,39 +1630,40 @@ __global__ void __launch_bounds__(128) paged_join_tile_kernel(const PagedAttnPar
     pdl_launch_dependents();
     pdl_wait();
   }
-  const int4 h = reinterpret_cast<const int4*>(p.ws)[blockIdx.x];
-  if (h.w == 0) return;
+  const PaHeader h = reinterpret_cast<const PaHeader*>(p.ws)[blockIdx.x];
+  if (h.parts == 0) return;
   constexpr int ROWS = pt_rows(D), COLS = D / 32;  // grid.y = 32 columns of 128 rows
-  const PaRequest r = pa_request(p, h.x);
-  const int t = blockIdx.y / COLS, c = blockIdx.y % COLS, row = threadIdx.x, half = 128 / p.ratio * p.ratio;
-  const int local = t * half + row, grow = h.z * p.tile_rows + local;
-  if (row >= half || grow >= r.n * p.ratio) return;
+  const int t = blockIdx.y / COLS, c = blockIdx.y % COLS, row = threadIdx.x, half = 128 / p.ratio * p.ratio, local = t * half + row;
+  if (row >= half || local >= h.rows) return;
   const uint8_t* parts = p.ws + pa_header_bytes(ctas);
   auto part = [&](int i) {  // the i-th part of the tile
     return reinterpret_cast<const float4*>(parts + (2ll * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * pa_part_bytes<ROWS, D>());
   };
   auto stat = [&](int i) { return reinterpret_cast<const float*>(part(i) + ROWS * D / 4) + t * 128 + row; };
   float top = -INFINITY;
-  for (int i = 0; i < h.w; ++i) top = fmaxf(top, *stat(i));
+#pragma unroll 4
+  for (int i = 0; i < h.parts; ++i) top = fmaxf(top, *stat(i));
   if (top == -INFINITY) top = 0.f;
   float sum = 0.f;
   uint32_t o[32] = {};
-#pragma unroll 1
-  for (int i = 0; i < h.w; ++i) {
+#pragma unroll 2
+  for (int i = 0; i < h.parts; ++i) {
+    const float4* src = part(i) + (t * (D / 4) + c * 8) * 128 + row;
+    float4 a[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a[e] = src[e * 128];
     const float f = pa_exp2(*stat(i) - top);
     sum += f * stat(i)[ROWS];
-    const float4* src = part(i) + (t * (D / 4) + c * 8) * 128 + row;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float4 a = src[e * 128];
-      o[4 * e] = __float_as_uint(__uint_as_float(o[4 * e]) + f * a.x);
-      o[4 * e + 1] = __float_as_uint(__uint_as_float(o[4 * e + 1]) + f * a.y);
-      o[4 * e + 2] = __float_as_uint(__uint_as_float(o[4 * e + 2]) + f * a.z);
-      o[4 * e + 3] = __float_as_uint(__uint_as_float(o[4 * e + 3]) + f * a.w);
+      o[4 * e] = __float_as_uint(__uint_as_float(o[4 * e]) + f * a[e].x);
+      o[4 * e + 1] = __float_as_uint(__uint_as_float(o[4 * e + 1]) + f * a[e].y);
+      o[4 * e + 2] = __float_as_uint(__uint_as_float(o[4 * e + 2]) + f * a[e].z);
+      o[4 * e + 3] = __float_as_uint(__uint_as_float(o[4 * e + 3]) + f * a[e].w);
     }
   }
-  const int token = grow / p.ratio;
-  pt_store32(p, (r.start + token) * p.ld_out + static_cast<long long>(h.y * p.ratio + grow - token * p.ratio) * D + c * 32, o, sum == 0.f ? 0.f : 1.f / sum);
+  const int grow = h.first + local, token = grow / p.ratio;
+  pt_store32(p, static_cast<long long>(h.start + token) * p.ld_out + static_cast<long long>(h.g * p.ratio + grow - token * p.ratio) * D + c * 32, o, sum == 0.f ? 0.f : 1.f / sum);
 }
 
 // The same for the sixteen-row form; a warp per row.
@@ -1458,23 +1673,23 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnParams p
     pdl_launch_dependents();
     pdl_wait();
   }
-  const int4 h = reinterpret_cast<const int4*>(p.ws)[blockIdx.x];
-  if (h.w == 0) return;
-  const PaRequest r = pa_request(p, h.x);
+  const PaHeader h = reinterpret_cast<const PaHeader*>(p.ws)[blockIdx.x];
+  if (h.parts == 0) return;
   const uint8_t* parts = p.ws + pa_header_bytes(ctas);
   auto part = [&](int i) {  // the i-th part of the tile
     return reinterpret_cast<const float*>(parts + (2ll * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * pa_part_bytes<ROWS, D>());
   };
-  const int lane = threadIdx.x & 31, rows = min(p.tile_rows, r.n * p.ratio - h.z * p.tile_rows);
-  for (int row = blockIdx.y * 4 + (threadIdx.x >> 5); row < rows; row += gridDim.y * 4) {
+  const int lane = threadIdx.x & 31;
+  for (int row = blockIdx.y * 4 + (threadIdx.x >> 5); row < h.rows; row += gridDim.y * 4) {
     float top = -INFINITY;
-    for (int i = lane; i < h.w; i += 32) top = fmaxf(top, part(i)[ROWS * D + row]);
+    for (int i = lane; i < h.parts; i += 32) top = fmaxf(top, part(i)[ROWS * D + row]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (top == -INFINITY) top = 0.f;
     constexpr int N = D / 32;
     float sum = 0.f, v[N] = {};
-    for (int i = 0; i < h.w; ++i) {
+#pragma unroll 4
+    for (int i = 0; i < h.parts; ++i) {
       const float* src = part(i);
       const float f = pa_exp2(src[ROWS * D + row] - top);
       sum += f * src[ROWS * D + ROWS + row];
@@ -1485,8 +1700,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnParams p
       }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int grow = h.z * p.tile_rows + row, token = grow / p.ratio;
-    const long long at = (r.start + token) * p.ld_out + static_cast<long long>(h.y * p.ratio + grow - token * p.ratio) * D;
+    const int grow = h.first + row, token = grow / p.ratio;
+    const long long at = static_cast<long long>(h.start + token) * p.ld_out + static_cast<long long>(h.g * p.ratio + grow - token * p.ratio) * D;
     float o[8];  // eight channels by one lane: its own, or (four channels per lane) its own and its neighbour's
 #pragma unroll
     for (int e = 0; e < N; ++e) o[e] = v[e] * inv;
@@ -1503,6 +1718,31 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnParams p
 // ------------------------------------------------------------------------------------------------ host
 // Which form: the rows of a key head that the largest request is known to bring.
 static bool pa_tile_form(int ratio, int max_tokens) { return ratio <= 128 && static_cast<long long>(ratio) * max_tokens > PR_ROWS; }
+// Whether clusters take the tiles: CTAs of a cluster per tile, or 0.  All tiles that these sizes allow must run at once, and even a full cache must
+// take a cluster no longer than an even share of all tiles and the joining of its parts would take all CTAs.
+template <class Kernel, int D>
+static int pa_clusters(Kernel* kernel, int threads, int smem, int size) {  // of `size` CTAs that the device holds at once
+  static host::DeviceCache cache[9];
+  return host::per_device(cache[size], [&] {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      n = 1;
+    }
+    return n;
+  });
+}
 static int pa_form_rows(int D, bool tiles) { return tiles ? pt_rows(D) : PR_ROWS; }
 
 static size_t pa_workspace(int D, bool tiles, int ctas) {
@@ -1510,13 +1750,14 @@ static size_t pa_workspace(int D, bool tiles, int ctas) {
 }
 
 using PaRowsKernel = void(const PagedAttnParams);
+using PaTileKernel = void(const CUtensorMap, const CUtensorMap, const CUtensorMap, const PagedAttnParams);
 using PaJoinKernel = void(const PagedAttnParams, int);
 
 static int pa_set_attributes() {
   static host::DeviceCache ready;
   const int set = host::per_device(ready, [] {
     const auto smem = [](auto* kernel, int bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess; };
-    return smem(paged_rows_kernel<128>, PR_SMEM) && smem(paged_rows_kernel<256>, PR_SMEM) && smem(paged_pair_kernel, PT_SMEM) && smem(paged_wide_kernel, PT_SMEM);
+    return smem(paged_rows_kernel<128>, pr_smem(128)) && smem(paged_rows_kernel<256>, pr_smem(256)) && smem(paged_pair_kernel, PT_SMEM) && smem(paged_wide_kernel, PT_SMEM);
   });
   return set ? TYBOK_OK : host::fail_cuda("paged_attention: shared memory");
 }
@@ -1536,7 +1777,8 @@ extern "C" {
 size_t tybok_paged_attention_workspace_bytes(int H, int G, int D, int max_tokens) {
   using namespace tb;
   if (H <= 0 || G <= 0 || max_tokens <= 0 || (D != 128 && D != 256)) return 0;
-  return pa_workspace(D, pa_tile_form(H / G, max_tokens), host::sm_count());
+  const bool tiles = pa_tile_form(H / G, max_tokens);
+  return pa_workspace(D, tiles, host::sm_count() * (tiles ? 1 : pr_ctas(D)));
 }
 
 int tybok_paged_attention(const void* q, int64_t ldq, const void* k_pages, const int64_t* k_strides, const void* v_pages,
@@ -1598,26 +1840,43 @@ int tybok_paged_attention(const void* q, int64_t ldq, const void* k_pages, const
     if (int rc = pa_pool_map(&tm_v, v_pages, v_strides, num_pages, G, page_size, D)) return rc;
   }
   if (int rc = pa_set_attributes()) return rc;
-  const int ctas = host::sm_count();
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  const int sms = host::sm_count(), threads = tiles ? PT_THREADS : PR_THREADS, smem = tiles ? PT_SMEM : pr_smem(D);
+  PaTileKernel* tile_kernel = D == 256 ? paged_wide_kernel : paged_pair_kernel;
+  PaRowsKernel* rows_kernel = D == 256 ? paged_rows_kernel<256> : paged_rows_kernel<128>;
+  // Tiles at most (a request's last one may be partly empty), key blocks of a full cache.
+  const double items = G * (B + std::floor(static_cast<double>(tokens) * p.ratio / p.tile_rows));
+  const double blocks = static_cast<double>(table_width) * page_size / (tiles ? pt_bk(D) : PR_BLOCK);
+  for (int size = 8; size >= 2 && !p.cluster; size /= 2) {
+    if (items * size > sms || blocks * (1.0 / size - items / sms) > p.join_blocks) continue;
+    const int room = tiles ? (D == 256 ? pa_clusters<PaTileKernel, 256>(tile_kernel, threads, smem, size) : pa_clusters<PaTileKernel, 128>(tile_kernel, threads, smem, size))
+                           : (D == 256 ? pa_clusters<PaRowsKernel, 256>(rows_kernel, threads, smem, size) : pa_clusters<PaRowsKernel, 128>(rows_kernel, threads, smem, size));
+    if (items <= room) p.cluster = size;
+  }
+  const int ctas = p.cluster ? static_cast<int>(items) * p.cluster : tiles ? sms : sms * pr_ctas(D);
+  cudaLaunchAttribute attr[2];
+  int na = 0;
+  if (p.pdl) {
+    attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[na++].val.programmaticStreamSerializationAllowed = 1;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(tiles ? PT_THREADS : PR_THREADS);
-  cfg.dynamicSmemBytes = tiles ? PT_SMEM : PR_SMEM;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cfg.attrs = attr;
-  cfg.numAttrs = p.pdl;
-  cudaError_t e;
-  if (tiles) {
-    e = cudaLaunchKernelEx(&cfg, D == 256 ? paged_wide_kernel : paged_pair_kernel, tm_q, tm_k, tm_v, p);
-  } else {
-    PaRowsKernel* kernel = D == 256 ? paged_rows_kernel<256> : paged_rows_kernel<128>;
-    e = cudaLaunchKernelEx(&cfg, kernel, p);
+  cfg.numAttrs = na;
+  if (p.cluster) {
+    attr[na].id = cudaLaunchAttributeClusterDimension;
+    attr[na].val.clusterDim.x = p.cluster;
+    attr[na].val.clusterDim.y = 1;
+    attr[na].val.clusterDim.z = 1;
+    cfg.numAttrs = na + 1;
   }
+  const cudaError_t e = tiles ? cudaLaunchKernelEx(&cfg, tile_kernel, tm_q, tm_k, tm_v, p) : cudaLaunchKernelEx(&cfg, rows_kernel, p);
   if (e != cudaSuccess) return host::fail_cuda("launch paged_attention");
   host::count_launch();
+  if (p.cluster) return TYBOK_OK;
   cfg.gridDim = dim3(ctas, tiles ? 8 : PR_ROWS / 4);  // tile forms: 128 rows x 32 columns each
   cfg.blockDim = dim3(128);
   cfg.dynamicSmemBytes = 0;
