@@ -738,7 +738,7 @@ struct __align__(16) PtBars {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t s_full[2];            // pair: per tile; wide: per score buffer
   uint64_t p_full[2][4];         // the same, and 32 of the block's keys
-  uint64_t done[4];              // pair: per tile, its last product has landed; wide: [block % 4], the block's product has
+  uint64_t done[2];              // pair: per tile, its last product has landed; wide: [block % 2], the block's product has
   uint64_t o_free;        // wide: the output of a tile has been read
   uint64_t pub[2][4];     // wide: per group and warp: the reference maximum after this block; at the end of a tile, its sums
   uint64_t fin[2][4];
@@ -1091,7 +1091,6 @@ __device__ __forceinline__ PaShare pt_begin(const PagedAttnParams& p, PtBars& ba
     for (int i = 0; i < 4; ++i) {
       mbar_init(&bars.piece_full[i], 1);
       mbar_init(&bars.piece_read[i], 11);  // eight softmax warps, keys, values, products
-      mbar_init(&bars.done[i], 1);
       for (int w = 0; w < 2; ++w) {
         mbar_init(&bars.p_full[w][i], 4);
         mbar_init(&bars.pub[w][i], 1);
@@ -1101,6 +1100,7 @@ __device__ __forceinline__ PaShare pt_begin(const PagedAttnParams& p, PtBars& ba
 #pragma unroll 1
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.done[i], 1);
       mbar_init(&bars.k_full[i], 1);
       mbar_init(&bars.k_empty[i], 1);
       mbar_init(&bars.v_full[i], 1);
@@ -1179,12 +1179,15 @@ __device__ __forceinline__ void pt_hand_over(bool live, uint64_t* handed) {
 }
 
 // The CTAs of a cluster join their parts of a tile, each for its share of the rows: a thread per row and 32 columns, parts in their order.
-// All of the CTA's work on its own part is done and visible to its threads.
+// By the softmax warps, which have the registers, between the two meetings of all threads of the cluster (pt_meet).
+__device__ __forceinline__ void pt_meet() {
+  __syncwarp();
+  cluster_arrive_release();
+  cluster_wait_acquire();
+}
 template <int D>
 __device__ __forceinline__ void pt_join(const PagedAttnParams& p, PtBars& bars, const float4* part) {
-  if (bars.item.rows == 0) return;  // no tile for the whole cluster
-  cluster_sync_all();
-  if (threadIdx.x >= 128) {  // (the warps with registers)
+  if (bars.item.rows > 0) {
     const int each = pt_rows(D) / p.cluster, rank = cluster_ctarank(), half = p.tile_rows / (pt_rows(D) / 128);
     for (int i = threadIdx.x - 128; i < each * (D / 32); i += 256) {
       const int at = rank * each + i % each, c = i / each, t = at >> 7, local = t * half + (at & 127);
@@ -1198,19 +1201,28 @@ __device__ __forceinline__ void pt_join(const PagedAttnParams& p, PtBars& bars, 
 #pragma unroll
       for (int k = 0; k < 8; ++k) top = fmaxf(top, m[k]);
       uint32_t o[32] = {};
+      const float4* src = part + (t * (D / 4) + c * 8) * 128 + (at & 127);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (m[k] == -INFINITY) continue;
-        const float f = pa_exp2(m[k] - top);
-        sum += f * l[k];
-        const float4* src = part + (t * (D / 4) + c * 8) * 128 + (at & 127);
+      for (int k0 = 0; k0 < 8; k0 += 4) {  // four peers' 32 channels on their way at once: a load takes 300 clocks and more
+        if (k0 >= p.cluster) break;
+        float4 a[4][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float4 a = pa_peer4(src + e * 128, k);
-          o[4 * e] = __float_as_uint(__uint_as_float(o[4 * e]) + f * a.x);
-          o[4 * e + 1] = __float_as_uint(__uint_as_float(o[4 * e + 1]) + f * a.y);
-          o[4 * e + 2] = __float_as_uint(__uint_as_float(o[4 * e + 2]) + f * a.z);
-          o[4 * e + 3] = __float_as_uint(__uint_as_float(o[4 * e + 3]) + f * a.w);
+        for (int k = 0; k < 4; ++k)
+          if (k0 + k < p.cluster)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) a[k][e] = pa_peer4(src + e * 128, k0 + k);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (m[k0 + k] == -INFINITY) continue;
+          const float f = pa_exp2(m[k0 + k] - top);
+          sum += f * l[k0 + k];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            o[4 * e] = __float_as_uint(__uint_as_float(o[4 * e]) + f * a[k][e].x);
+            o[4 * e + 1] = __float_as_uint(__uint_as_float(o[4 * e + 1]) + f * a[k][e].y);
+            o[4 * e + 2] = __float_as_uint(__uint_as_float(o[4 * e + 2]) + f * a[k][e].z);
+            o[4 * e + 3] = __float_as_uint(__uint_as_float(o[4 * e + 3]) + f * a[k][e].w);
+          }
         }
       }
       const int ahead = local / p.ratio;
@@ -1218,8 +1230,6 @@ __device__ __forceinline__ void pt_join(const PagedAttnParams& p, PtBars& bars, 
                  sum == 0.f ? 0.f : 1.f / sum);
     }
   }
-  __syncwarp();
-  cluster_sync_all();  // nobody's part is read any more
 }
 
 __global__ void __launch_bounds__(PT_THREADS, 1)
@@ -1316,6 +1326,10 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       }
       mbar_wait(&bars.mma_done, 0);
     }
+    if (p.cluster) {
+      pt_meet();  // every CTA has left its part
+      pt_meet();  // nobody's part is read any more
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_REGS_SOFTMAX));
     const int t = (warp - 4) >> 2, q = warp & 3, row = q * 32 + lane;
@@ -1384,6 +1398,11 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       bars.abort = 1;
       if (p.status) atomicCAS(p.status, 0, TYBOK_DEV_TIMEOUT_EPILOGUE);
     }
+    if (p.cluster) {
+      pt_meet();
+      pt_join<D>(p, bars, reinterpret_cast<const float4*>(sk));
+      pt_meet();
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -1391,7 +1410,6 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  if (p.cluster) pt_join<D>(p, bars, reinterpret_cast<const float4*>(sk));
 }
 
 __global__ void __launch_bounds__(PT_THREADS, 1)
@@ -1413,7 +1431,8 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       pt_lead<D>(p, first, share, &tm_q, sq, bars);
     } else if (warp != 1) {
       const bool k = warp == 0;
-      const PtRing rings[1] = {{k ? &tm_k : &tm_v, k ? sk : sv, k ? bars.k_full : bars.v_full, k ? bars.k_empty : bars.v_empty}};
+      // a key block's place is free when its scores are there, a value block's when its product is: no barriers of their own
+      const PtRing rings[1] = {{k ? &tm_k : &tm_v, k ? sk : sv, k ? bars.k_full : bars.v_full, k ? bars.s_full : bars.done}};
       pt_stream<D, 1>(p, rings, bars);
     } else {
       const uint32_t leader = elect_one();
@@ -1472,13 +1491,9 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
               pt_mma_ts(leader, tmem + s * 64, tmem + 128 + ks * 8, k_desc + o, idesc_s, ks > 0 ? 1u : 0u);
             }
             pt_commit(leader, &bars.s_full[s]);
-            pt_commit(leader, &bars.k_empty[s]);
             if (j + 3 == nb) pt_commit(leader, &bars.q_used);  // the last scores have been issued
           }
-          if (j >= 0) {
-            pt_commit(leader, &bars.done[vb & 3]);
-            pt_commit(leader, &bars.v_empty[s]);
-          }
+          if (j >= 0) pt_commit(leader, &bars.done[s]);
         }
         i += nb;
       }
@@ -1489,6 +1504,10 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (p.status) atomicCAS(p.status, 0, TYBOK_DEV_TIMEOUT_MMA);
       }
       mbar_wait(&bars.mma_done, 0);
+    }
+    if (p.cluster) {
+      pt_meet();  // every CTA has left its part
+      pt_meet();  // nobody's part is read any more
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_REGS_SOFTMAX));
@@ -1563,7 +1582,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           if (__any_sync(0xffffffffu, grow) && j > at.blk) {
             // The product before must have landed.  (These scores came after that of two blocks ago, so the barrier's phase before has
             // passed, and its next waits for this block's weights.)
-            if (!wait(&bars.done[(i - 1) & 3], ((i - 1) >> 2) & 1)) break;
+            if (!wait(&bars.done[(i - 1) & 1], ((i - 1) >> 1) & 1)) break;
             tc_fence_after();
             pt_rescale(t_o, 8, grow ? pa_exp2(m_ref - m_blk) : 1.0f);
           }
@@ -1583,7 +1602,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       if (!wait(&bars.fin[grp ^ 1][q], n & 1)) break;
       const float m_other = bars.end_m[n & 1][grp ^ 1][row], m_end = fmaxf(m_own, m_other);
       l = l * pa_exp2(m_own - m_end) + bars.end_l[n & 1][grp ^ 1][row] * pa_exp2(m_other - m_end);
-      if (!wait(&bars.done[(i - 1) & 3], ((i - 1) >> 2) & 1)) break;
+      if (!wait(&bars.done[(i - 1) & 1], ((i - 1) >> 1) & 1)) break;
       if (live) {
         tc_fence_after();
         const float inv = at.part ? 1.f : l == 0.f ? 0.f : 1.f / l;
@@ -1613,6 +1632,11 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       bars.abort = 1;
       if (p.status) atomicCAS(p.status, 0, TYBOK_DEV_TIMEOUT_EPILOGUE);
     }
+    if (p.cluster) {
+      pt_meet();
+      pt_join<D>(p, bars, reinterpret_cast<const float4*>(sk));
+      pt_meet();
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -1620,7 +1644,6 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  if (p.cluster) pt_join<D>(p, bars, reinterpret_cast<const float4*>(sk));
 }
 
 // Joins the parts of the tile that CTA blockIdx.x of a tile form began: a thread per row and 32 columns.
@@ -1829,7 +1852,7 @@ int tybok_paged_attention(const void* q, int64_t ldq, const void* k_pages, const
   const double most_tiles = static_cast<double>(tokens) * p.ratio / p.tile_rows + B, most_blocks = static_cast<double>(table_width) * page_size / 64 + 1;
   if (most_tiles * G * most_blocks > 4e9) return host::fail(TYBOK_ERR_ARG, "paged_attention: more than 2^32 key blocks could fall to one call");
   p.tile_tokens = p.tile_rows % p.ratio == 0 ? p.tile_rows / p.ratio : 0;
-  p.join_blocks = tiles ? (D == 128 ? 3 : 6) : 4;
+  p.join_blocks = tiles ? (D == 128 ? 3 : 9) : 4;
   CUtensorMap tm_q, tm_k, tm_v;
   if (tiles) {
     const uint64_t dims[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(p.ratio), static_cast<uint64_t>(G), static_cast<uint64_t>(tokens)};
