@@ -357,21 +357,11 @@ __device__ PaShare pa_share(const PagedAttnParams& p, PaPlace& first) {
   first = next;
   return sh;
 }
-__device__ __forceinline__ float4 pa_peer4(const void* local, int rank) {  // 16 bytes of another CTA of the cluster
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(dsmem_addr(smem_u32(local), rank)));
-  return v;
-}
-__device__ __forceinline__ void pa_send4(const void* local, int rank, float4 v) {
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dsmem_addr(smem_u32(local), rank)), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+__device__ __forceinline__ void pa_send4(uint32_t to, float4 v) {  // to another CTA of the cluster
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 __device__ __forceinline__ void pa_send(const void* local, int rank, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dsmem_addr(smem_u32(local), rank)), "f"(v) : "memory");
-}
-__device__ __forceinline__ float pa_peer(const void* local, int rank) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(dsmem_addr(smem_u32(local), rank)));
-  return v;
 }
 
 // How many CTAs the tile has that begins at x in this CTA's share and goes on behind it.
@@ -604,8 +594,9 @@ __global__ void __launch_bounds__(PR_THREADS, pr_ctas(D)) paged_rows_kernel(cons
         pa_store8(p, (at.r.start + token) * p.ld_out + static_cast<long long>(at.g * p.ratio + grow - token * p.ratio) * D + c, v);
       } else if (p.cluster) {
         const int owner = row / each, at_owner = rank * each + row % each;
-        pa_send4(parts + at_owner * D + c, owner, make_float4(v[0], v[1], v[2], v[3]));
-        pa_send4(parts + at_owner * D + c + 4, owner, make_float4(v[4], v[5], v[6], v[7]));
+        const uint32_t to = dsmem_addr(smem_u32(parts + at_owner * D + c), owner);
+        pa_send4(to, make_float4(v[0], v[1], v[2], v[3]));
+        pa_send4(to + 16, make_float4(v[4], v[5], v[6], v[7]));
         if (c == 0) {
           pa_send(parts + PR_ROWS * D + at_owner, owner, top);
           pa_send(parts + PR_ROWS * D + PR_ROWS + at_owner, owner, sum);
@@ -1115,7 +1106,6 @@ __device__ __forceinline__ PaShare pt_begin(const PagedAttnParams& p, PtBars& ba
     bars.abort = 0;
     fence_barrier_init();
   }
-  if (p.cluster && tid >= 128) bars.part_m[tid - 128] = -INFINITY;
   if (warp == 1) {
     tmem_alloc(&bars.tmem_base, 512);
     tmem_relinquish();
@@ -1178,57 +1168,69 @@ __device__ __forceinline__ void pt_hand_over(bool live, uint64_t* handed) {
   }
 }
 
-// The CTAs of a cluster join their parts of a tile, each for its share of the rows: a thread per row and 32 columns, parts in their order.
-// By the softmax warps, which have the registers, between the two meetings of all threads of the cluster (pt_meet).
+// The CTAs of a cluster join their parts of a tile. Each owns a share of the rows; once all have left their rings, the softmax warps send
+// every row's part, from tensor memory, to its owner: [part][column / 4][row of the share], over the ring. With everything here the owner
+// adds the parts up in their order, a thread per row and 32 columns. (All threads of the cluster meet before and after the sending.)
 __device__ __forceinline__ void pt_meet() {
   __syncwarp();
   cluster_arrive_release();
   cluster_wait_acquire();
 }
+// chunks [c0, c1) of 32 columns of tile t's `row`; m = -INFINITY: no part of it here
 template <int D>
-__device__ __forceinline__ void pt_join(const PagedAttnParams& p, PtBars& bars, const float4* part) {
-  if (bars.item.rows > 0) {
-    const int each = pt_rows(D) / p.cluster, rank = cluster_ctarank(), half = p.tile_rows / (pt_rows(D) / 128);
-    for (int i = threadIdx.x - 128; i < each * (D / 32); i += 256) {
-      const int at = rank * each + i % each, c = i / each, t = at >> 7, local = t * half + (at & 127);
-      if ((at & 127) >= half || local >= bars.item.rows) continue;
-      float m[8], l[8], top = -INFINITY, sum = 0.f;
+__device__ __forceinline__ void pt_send(const PagedAttnParams& p, PtBars& bars, float4* parts, uint32_t t_o, int t, int row, int c0, int c1, bool live, bool mine, float m, float l) {
+  const int each = pt_rows(D) / p.cluster, at = t * 128 + row, owner = at / each, here = at - owner * each, rank = cluster_ctarank();
+  if (c0 == 0) {
+    pa_send(&bars.part_m[rank * each + here], owner, mine ? m : -INFINITY);
+    pa_send(&bars.part_l[rank * each + here], owner, l);
+  }
+  if (!live) return;
+  const uint32_t to = dsmem_addr(smem_u32(parts + rank * (D / 4) * each + here), owner), step = each * 16;
+  tc_fence_after();
+#pragma unroll 1
+  for (int c = c0; c < c1; ++c) {
+    uint32_t o[32];
+    tmem_ld32(t_o + c * 32, o);
+    tc_wait_ld();
+    if (mine)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        m[k] = k < p.cluster ? pa_peer(&bars.part_m[at], k) : -INFINITY;  // (of a CTA without blocks, too)
-        l[k] = k < p.cluster ? pa_peer(&bars.part_l[at], k) : 0.f;
-      }
+      for (int e = 0; e < 8; ++e)
+        pa_send4(to + (c * 8 + e) * step, make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3])));
+  }
+}
+template <int D>
+__device__ __forceinline__ void pt_join(const PagedAttnParams& p, const PtBars& bars, const float4* parts) {
+  if (bars.item.rows == 0) return;
+  const int each = pt_rows(D) / p.cluster, rank = cluster_ctarank(), half = p.tile_rows / (pt_rows(D) / 128);
+  for (int i = threadIdx.x - 128; i < each * (D / 32); i += 256) {
+    const int here = i % each, at = rank * each + here, c = i / each, local = (at >> 7) * half + (at & 127);
+    if ((at & 127) >= half || local >= bars.item.rows) continue;
+    float m[8], top = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) top = fmaxf(top, m[k]);
-      uint32_t o[32] = {};
-      const float4* src = part + (t * (D / 4) + c * 8) * 128 + (at & 127);
-#pragma unroll
-      for (int k0 = 0; k0 < 8; k0 += 4) {  // four peers' 32 channels on their way at once: a load takes 300 clocks and more
-        if (k0 >= p.cluster) break;
-        float4 a[4][8];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (k0 + k < p.cluster)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) a[k][e] = pa_peer4(src + e * 128, k0 + k);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (m[k0 + k] == -INFINITY) continue;
-          const float f = pa_exp2(m[k0 + k] - top);
-          sum += f * l[k0 + k];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            o[4 * e] = __float_as_uint(__uint_as_float(o[4 * e]) + f * a[k][e].x);
-            o[4 * e + 1] = __float_as_uint(__uint_as_float(o[4 * e + 1]) + f * a[k][e].y);
-            o[4 * e + 2] = __float_as_uint(__uint_as_float(o[4 * e + 2]) + f * a[k][e].z);
-            o[4 * e + 3] = __float_as_uint(__uint_as_float(o[4 * e + 3]) + f * a[k][e].w);
-          }
-        }
-      }
-      const int ahead = local / p.ratio;
-      pt_store32(p, static_cast<long long>(bars.item.token + ahead) * p.ld_out + static_cast<long long>(bars.item.g * p.ratio + local - ahead * p.ratio) * D + c * 32, o,
-                 sum == 0.f ? 0.f : 1.f / sum);
+    for (int k = 0; k < 8; ++k) {
+      m[k] = k < p.cluster ? bars.part_m[k * each + here] : -INFINITY;
+      top = fmaxf(top, m[k]);
     }
+    uint32_t o[32] = {};
+#pragma unroll 1
+    for (int k = 0; k < p.cluster; ++k) {
+      const float mk = bars.part_m[k * each + here];
+      if (mk == -INFINITY) continue;
+      const float f = pa_exp2(mk - top);
+      sum += f * bars.part_l[k * each + here];
+      const float4* src = parts + (k * (D / 4) + c * 8) * each + here;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float4 a = src[e * each];
+        o[4 * e] = __float_as_uint(__uint_as_float(o[4 * e]) + f * a.x);
+        o[4 * e + 1] = __float_as_uint(__uint_as_float(o[4 * e + 1]) + f * a.y);
+        o[4 * e + 2] = __float_as_uint(__uint_as_float(o[4 * e + 2]) + f * a.z);
+        o[4 * e + 3] = __float_as_uint(__uint_as_float(o[4 * e + 3]) + f * a.w);
+      }
+    }
+    const int ahead = local / p.ratio;
+    pt_store32(p, static_cast<long long>(bars.item.token + ahead) * p.ld_out + static_cast<long long>(bars.item.g * p.ratio + local - ahead * p.ratio) * D + c * 32, o,
+               sum == 0.f ? 0.f : 1.f / sum);
   }
 }
 
@@ -1327,8 +1329,8 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       mbar_wait(&bars.mma_done, 0);
     }
     if (p.cluster) {
-      pt_meet();  // every CTA has left its part
-      pt_meet();  // nobody's part is read any more
+      pt_meet();
+      pt_meet();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_REGS_SOFTMAX));
@@ -1341,6 +1343,7 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     pa_zero_rows<D>(p, tid - 128, 256);
     uint32_t n = 0, i = 0;  // tiles and blocks of this group
     bool ok = true;
+    float part_m = -INFINITY, part_l = 0.f;  // cluster: of this row
     PtReader reader;
     PtPiece at{};
     while (ok && reader.next(bars, at)) {
@@ -1371,11 +1374,15 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       }
       ok = ok && __all_sync(0xffffffffu, wait_or_abort(&bars.done[t], n & 1, &bars.abort));
       ++n;
+      if (p.cluster) {
+        if (ok) part_m = m_ref, part_l = l;
+        break;  // the only piece
+      }
       if (ok && live) {
         tc_fence_after();
         const float inv = at.part ? 1.f : l == 0.f ? 0.f : 1.f / l;
         // [tile][column / 4][row], then the references and sums of both tiles
-        float4* part = p.cluster ? reinterpret_cast<float4*>(sk) : reinterpret_cast<float4*>(p.ws + pa_header_bytes(gridDim.x) + (2ll * blockIdx.x + at.part - 1) * pa_part_bytes<pt_rows(D), D>());
+        float4* part = reinterpret_cast<float4*>(p.ws + pa_header_bytes(gridDim.x) + (2ll * blockIdx.x + at.part - 1) * pa_part_bytes<pt_rows(D), D>());
         const long long to = static_cast<long long>(at.token + ahead) * p.ld_out + static_cast<long long>(at.g * p.ratio + local - ahead * p.ratio) * D;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
@@ -1387,8 +1394,8 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         }
         if (at.part) {
           float* stat = reinterpret_cast<float*>(part + pt_rows(D) * D / 4);
-          (p.cluster ? bars.part_m : stat)[t * 128 + row] = m_ref;
-          (p.cluster ? bars.part_l : stat + pt_rows(D))[t * 128 + row] = l;
+          stat[t * 128 + row] = m_ref;
+          stat[pt_rows(D) + t * 128 + row] = l;
         }
         tc_fence_before();
       }
@@ -1399,9 +1406,11 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       if (p.status) atomicCAS(p.status, 0, TYBOK_DEV_TIMEOUT_EPILOGUE);
     }
     if (p.cluster) {
+      const int valid = at.rows - t * half;  // (no piece: no rows)
+      pt_meet();
+      pt_send<D>(p, bars, reinterpret_cast<float4*>(sk), t_o, t, row, 0, 4, q * 32 < valid && __any_sync(0xffffffffu, part_m > -INFINITY), row < valid, part_m, part_l);
       pt_meet();
       pt_join<D>(p, bars, reinterpret_cast<const float4*>(sk));
-      pt_meet();
     }
   }
   tc_fence_before();
@@ -1506,8 +1515,8 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       mbar_wait(&bars.mma_done, 0);
     }
     if (p.cluster) {
-      pt_meet();  // every CTA has left its part
-      pt_meet();  // nobody's part is read any more
+      pt_meet();
+      pt_meet();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_REGS_SOFTMAX));
@@ -1551,6 +1560,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     };
     PtReader reader;
     PtPiece at{}, next{};
+    float part_m = -INFINITY, part_l = 0.f;  // cluster: of this row
     bool any = reader.next(bars, at) && queries(0);
     pa_check(p, tid - 128, 256);
     pa_zero_rows<D>(p, tid - 128, 256);
@@ -1603,10 +1613,14 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const float m_other = bars.end_m[n & 1][grp ^ 1][row], m_end = fmaxf(m_own, m_other);
       l = l * pa_exp2(m_own - m_end) + bars.end_l[n & 1][grp ^ 1][row] * pa_exp2(m_other - m_end);
       if (!wait(&bars.done[(i - 1) & 1], ((i - 1) >> 1) & 1)) break;
+      if (p.cluster) {
+        part_m = m_end, part_l = l;
+        break;  // the only piece
+      }
       if (live) {
         tc_fence_after();
         const float inv = at.part ? 1.f : l == 0.f ? 0.f : 1.f / l;
-        float4* part = p.cluster ? reinterpret_cast<float4*>(sk) : reinterpret_cast<float4*>(p.ws + pa_header_bytes(gridDim.x) + (2ll * blockIdx.x + at.part - 1) * pa_part_bytes<pt_rows(D), D>());
+        float4* part = reinterpret_cast<float4*>(p.ws + pa_header_bytes(gridDim.x) + (2ll * blockIdx.x + at.part - 1) * pa_part_bytes<pt_rows(D), D>());
         const long long to = static_cast<long long>(at.token + ahead) * p.ld_out + static_cast<long long>(at.g * p.ratio + row - ahead * p.ratio) * D;
 #pragma unroll 1
         for (int c = 4 * grp; c < 4 * grp + 4; ++c) {
@@ -1618,8 +1632,8 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         }
         if (at.part && grp == 0) {
           float* stat = reinterpret_cast<float*>(part + pt_rows(D) * D / 4);
-          (p.cluster ? bars.part_m : stat)[row] = m_end;
-          (p.cluster ? bars.part_l : stat + pt_rows(D))[row] = l;
+          stat[row] = m_end;
+          stat[pt_rows(D) + row] = l;
         }
       }
       tc_fence_before();
@@ -1634,8 +1648,9 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     }
     if (p.cluster) {
       pt_meet();
-      pt_join<D>(p, bars, reinterpret_cast<const float4*>(sk));
+      pt_send<D>(p, bars, reinterpret_cast<float4*>(sk), t_o, 0, row, 4 * grp, 4 * grp + 4, q * 32 < at.rows && __any_sync(0xffffffffu, part_m > -INFINITY), row < at.rows, part_m, part_l);
       pt_meet();
+      pt_join<D>(p, bars, reinterpret_cast<const float4*>(sk));
     }
   }
   tc_fence_before();
