@@ -1402,8 +1402,8 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     }
     ok = ok && reader.ok;
     if (!ok && lane == 0) {
-      bars.abort = 1;
       if (p.status) atomicCAS(p.status, 0, TYBOK_DEV_TIMEOUT_EPILOGUE);
+      bars.abort = 1;
     }
     if (p.cluster) {
       const int valid = at.rows - t * half;  // (no piece: no rows)
@@ -1643,8 +1643,8 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     }
     ok = ok && reader.ok;
     if (!ok && lane == 0) {
-      bars.abort = 1;
       if (p.status) atomicCAS(p.status, 0, TYBOK_DEV_TIMEOUT_EPILOGUE);
+      bars.abort = 1;
     }
     if (p.cluster) {
       pt_meet();
