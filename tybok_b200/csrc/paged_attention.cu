@@ -47,6 +47,7 @@ struct PagedAttnParams {
   int tile_tokens;   // tokens of a tile where it holds whole ones, else 0
   int wide_out;      // the outputs are 32-byte aligned
   int join_blocks;   // what leaving a tile to two CTAs costs, in key blocks
+  int tile_blocks;   // what beginning and ending a tile costs, in key blocks
   int cluster;       // > 0: one row tile per cluster of that many CTAs, which share its key blocks and join their parts themselves
   float scale_log2e;     // softmax scale * log2(e), with its sign
   float abs_scale_log2e; // its magnitude, above zero, and the bit of the scores' instruction that negates Q instead
@@ -161,16 +162,18 @@ __device__ __forceinline__ void pa_store8(const PagedAttnParams& p, long long at
   }
 }
 
-// The line: the key blocks of all (request, key head, row tile), numbered in that order.  Whole warps ask, each for itself:
+// The line: the key blocks of all (request, key head, row tile), numbered in that order; where the shares are long enough for it to count,
+// each tile's are led by `extra` places that stand for its beginning and end.  Whole warps ask, each for itself:
 // request 32 k + lane at a time, and the sums of such groups stay in the lanes.
 struct PaGroup {      // 32 requests
   PaRequest r;        // this lane's
   int tiles;
-  uint32_t cost, sum; // blocks of one of its key heads; blocks of all of them up to this lane's request
+  uint32_t cost, sum; // places of one of its key heads; places of all of them up to this lane's request
 };
 struct PaLine {
-  uint32_t blocks, tiles;
-  uint32_t sums[PA_MAX_REQUESTS / 1024];  // blocks of group 32 i + lane
+  uint32_t places, tiles;
+  int longest, extra;                     // blocks of the longest tile
+  uint32_t sums[PA_MAX_REQUESTS / 1024];  // places of group 32 i + lane
   PaGroup last;
 };
 __device__ __forceinline__ uint32_t pa_scan(uint32_t x) {  // inclusive sums over the warp
@@ -202,13 +205,13 @@ __device__ __forceinline__ uint32_t pa_cost(const PagedAttnParams& p, const PaRe
   return cost;
 }
 template <int BK>
-__device__ __forceinline__ PaGroup pa_group(const PagedAttnParams& p, int k) {
+__device__ __forceinline__ PaGroup pa_group(const PagedAttnParams& p, int k, int extra) {
   const int b = 32 * k + (threadIdx.x & 31);
   PaGroup g;
   g.r = {0, 0, 0};
   if (b < p.B) g.r = pa_request(p, b);
   g.tiles = pa_tiles(p, g.r.n);
-  g.cost = pa_cost<BK>(p, g.r, g.tiles);
+  g.cost = pa_cost<BK>(p, g.r, g.tiles) + g.tiles * extra;
   g.sum = pa_scan(g.cost * p.G);
   return g;
 }
@@ -216,25 +219,36 @@ template <int BK>
 __device__ __forceinline__ PaLine pa_line(const PagedAttnParams& p) {
   const int lane = threadIdx.x & 31;
   PaLine line{};
+  uint32_t tiles[PA_MAX_REQUESTS / 1024] = {}, all_tiles = 0;  // up to this lane's request in the last group
 #pragma unroll 1
   for (int k = 0; 32 * k < p.B; ++k) {
-    line.last = pa_group<BK>(p, k);
-    const uint32_t sum = __shfl_sync(0xffffffffu, line.last.sum, 31);
+    line.last = pa_group<BK>(p, k, 0);
+    all_tiles = pa_scan(static_cast<uint32_t>(line.last.tiles) * p.G);
+    if (!p.cluster && line.last.tiles > 0) line.longest = max(line.longest, pa_blocks<BK>(p, line.last.r, line.last.tiles - 1));
+    const uint32_t sum = __shfl_sync(0xffffffffu, line.last.sum, 31), count = __shfl_sync(0xffffffffu, all_tiles, 31);
 #pragma unroll
     for (int i = 0; i < PA_MAX_REQUESTS / 1024; ++i)
-      if (k == 32 * i + lane) line.sums[i] = sum;
-    line.blocks += sum;
-    line.tiles += __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(line.last.tiles)) * p.G;
+      if (k == 32 * i + lane) line.sums[i] = sum, tiles[i] = count;
+    line.places += sum;
+    line.tiles += count;
   }
+  line.longest = __reduce_max_sync(0xffffffffu, line.longest);
+  if (p.cluster || line.places < p.tile_blocks * gridDim.x) return line;
+  line.extra = p.tile_blocks;
+  line.places += line.tiles * line.extra;
+#pragma unroll
+  for (int i = 0; i < PA_MAX_REQUESTS / 1024; ++i) line.sums[i] += tiles[i] * line.extra;
+  line.last.cost += line.last.tiles * line.extra;
+  line.last.sum += all_tiles * line.extra;
   return line;
 }
 
-// A place in the line: block `blk` of `nblk` of row tile `tile` of key head `g` of request `b`.
+// A place in the line: place `blk` of `nblk` of row tile `tile` of key head `g` of request `b`.
 struct PaPlace {
   int b, g, tile, blk, nblk, tiles;
   PaRequest r;
 };
-// Where block x < line.blocks lies.
+// Where place x < line.places lies.
 template <int BK>
 __device__ __forceinline__ PaPlace pa_locate(const PagedAttnParams& p, const PaLine& line, uint32_t x) {
   const int lane = threadIdx.x & 31;
@@ -253,12 +267,12 @@ __device__ __forceinline__ PaPlace pa_locate(const PagedAttnParams& p, const PaL
         break;
       }
     }
-    g = pa_group<BK>(p, k);
+    g = pa_group<BK>(p, k, line.extra);
   }
   const int src = __popc(__ballot_sync(0xffffffffu, g.sum <= x));
   const uint32_t per_head = __shfl_sync(0xffffffffu, g.cost, src);
   x -= __shfl_sync(0xffffffffu, g.sum, src) - per_head * p.G;
-  PaPlace at;
+  PaPlace at{};
   at.b = 32 * k + src;
   at.r = {__shfl_sync(0xffffffffu, g.r.start, src), __shfl_sync(0xffffffffu, g.r.n, src), __shfl_sync(0xffffffffu, g.r.len, src)};
   at.tiles = __shfl_sync(0xffffffffu, g.tiles, src);
@@ -271,14 +285,14 @@ __device__ __forceinline__ PaPlace pa_locate(const PagedAttnParams& p, const PaL
     return at;
   }
   if (!p.causal) {
-    at.nblk = max(1, (at.r.len + BK - 1) / BK);
+    at.nblk = max(1, (at.r.len + BK - 1) / BK) + line.extra;
     at.tile = static_cast<int>(x / at.nblk);
     at.blk = static_cast<int>(x) - at.tile * at.nblk;
     return at;
   }
 #pragma unroll 1
-  for (at.tile = 0;; at.tile += 32) {  // 32 tiles at a time
-    const uint32_t n = at.tile + lane < at.tiles ? pa_blocks<BK>(p, at.r, at.tile + lane) : 0, to = pa_scan(n);
+  for (at.tile = 0; at.tile < at.tiles; at.tile += 32) {  // 32 tiles at a time
+    const uint32_t n = at.tile + lane < at.tiles ? pa_blocks<BK>(p, at.r, at.tile + lane) + line.extra : 0, to = pa_scan(n);
     const uint32_t past = __ballot_sync(0xffffffffu, to <= x);
     if (past != 0xffffffffu) {
       const int i = __popc(past);
@@ -289,10 +303,11 @@ __device__ __forceinline__ PaPlace pa_locate(const PagedAttnParams& p, const PaL
     }
     x -= __shfl_sync(0xffffffffu, to, 31);
   }
+  return at;  // (not reached: x lies in the line)
 }
 // The tile after this one (the caller knows that there is one).
 template <int BK>
-__device__ __forceinline__ void pa_next(const PagedAttnParams& p, PaPlace& at) {
+__device__ __forceinline__ void pa_next(const PagedAttnParams& p, PaPlace& at, int extra) {
   if (++at.tile == at.tiles) {
     at.tile = 0;
     if (++at.g == p.G) {
@@ -305,25 +320,28 @@ __device__ __forceinline__ void pa_next(const PagedAttnParams& p, PaPlace& at) {
     }
   }
   at.blk = 0;
-  at.nblk = pa_blocks<BK>(p, at.r, at.tile);
+  at.nblk = pa_blocks<BK>(p, at.r, at.tile) + extra;
 }
 
-// A CTA's share [x0, x1) of the line: equal numbers of blocks, borders moved to the edge of a tile that lies near.  With `whole` every
-// border moves to the nearest edge, so no tile has two CTAs: where the rounds of whole tiles take no longer than an even
-// share and the joining of its parts.
+// A CTA's share [x0, x1) of the line: equal numbers of places, borders moved to the edge of a tile that lies near (and from a tile's
+// leading places to its beginning).  With `whole` every border moves to the nearest edge, so no tile has two CTAs: where the
+// rounds of whole tiles take no longer than an even share and the joining of its parts.
 struct PaShare {
   uint32_t per, x0, x1;
+  int extra;
   bool whole;
 };
 __device__ __forceinline__ int pa_snap(const PaShare& sh, int blk, int nblk, int join_blocks) {
   const bool up = 2 * blk > nblk;
   const int away = up ? nblk - blk : blk;
-  return sh.whole || 4 * away <= static_cast<int>(min(sh.per, 4u * join_blocks)) - 4 ? (up ? nblk : 0) : blk;
+  if (sh.whole || 4 * away <= static_cast<int>(min(sh.per, 4u * join_blocks)) - 4) return up ? nblk : 0;
+  return blk <= sh.extra ? 0 : blk;
 }
 template <int BK>
 __device__ PaShare pa_share(const PagedAttnParams& p, PaPlace& first) {
   const PaLine line = pa_line<BK>(p);
   PaShare sh;
+  sh.extra = line.extra;
   if (p.cluster) {  // tile number blockIdx.x / cluster; `per` blocks of it to each CTA
     sh.whole = false;
     sh.per = sh.x0 = sh.x1 = 0;
@@ -336,16 +354,15 @@ __device__ PaShare pa_share(const PagedAttnParams& p, PaPlace& first) {
     return sh;
   }
   const uint32_t ctas = gridDim.x;
-  sh.per = (line.blocks + ctas - 1) / ctas;
-  // rounds * average length of a tile against an even share
-  sh.whole = static_cast<float>((line.tiles + ctas - 1) / ctas) * line.blocks <= static_cast<float>(sh.per + p.join_blocks) * line.tiles;
+  sh.per = (line.places + ctas - 1) / ctas;
+  sh.whole = static_cast<float>((line.tiles + ctas - 1) / ctas) * (line.longest + line.extra) <= static_cast<float>(sh.per + p.join_blocks);
   PaPlace next{};
   uint32_t border[2];
 #pragma unroll 1
   for (int i = 1; i >= 0; --i) {
     const unsigned long long x = static_cast<unsigned long long>(blockIdx.x + i) * sh.per;
-    border[i] = line.blocks;
-    if (x >= line.blocks) continue;
+    border[i] = line.places;
+    if (x >= line.places) continue;
     next = pa_locate<BK>(p, line, static_cast<uint32_t>(x));
     const int blk = pa_snap(sh, next.blk, next.nblk, p.join_blocks);
     border[i] = static_cast<uint32_t>(x) - next.blk + blk;
@@ -353,7 +370,7 @@ __device__ PaShare pa_share(const PagedAttnParams& p, PaPlace& first) {
   }
   sh.x0 = border[0];
   sh.x1 = border[1];
-  if (sh.x0 < sh.x1 && next.blk == next.nblk) pa_next<BK>(p, next);
+  if (sh.x0 < sh.x1 && next.blk == next.nblk) pa_next<BK>(p, next, sh.extra);
   first = next;
   return sh;
 }
@@ -615,7 +632,7 @@ __global__ void __launch_bounds__(PR_THREADS, pr_ctas(D)) paged_rows_kernel(cons
     if (!whole_tile && at.blk == 0) header = {pa_parts(p, share, x, at.nblk), min(PR_ROWS, rows - at.tile * PR_ROWS), at.tile * PR_ROWS, at.r.start, at.g};
     x += end - at.blk;
     __syncthreads();  // the ring is free again
-    if (x < x1) pa_next<BK>(p, at);
+    if (x < x1) pa_next<BK>(p, at, 0);
   }
   if (!tidied) tidy();
   if (!p.cluster) {
@@ -871,19 +888,21 @@ __device__ __forceinline__ void pt_lead(const PagedAttnParams& p, PaPlace at, co
     if (n >= PT_PIECES) ok = __all_sync(0xffffffffu, wait_or_abort(&bars.piece_read[s], (n / PT_PIECES - 1) & 1, &bars.abort));
     if (!ok) break;
     const bool any = x < share.x1;
+    int end = 0;
     PtPiece w{};
     if (any) {
       const int first = at.tile * p.tile_tokens;
       w.rows = min(p.tile_rows, at.r.n * p.ratio - at.tile * p.tile_rows);
       w.b = at.b;
       w.g = at.g;
-      w.blk = at.blk;
-      w.end = static_cast<int>(min(static_cast<uint32_t>(at.nblk), at.blk + (share.x1 - x)));
+      end = static_cast<int>(min(static_cast<uint32_t>(at.nblk), at.blk + (share.x1 - x)));
+      w.blk = max(0, at.blk - share.extra);
+      w.end = end - share.extra;
       w.len = at.r.len;
       w.seen = p.causal ? at.r.len - at.r.n + first + 1 : at.r.len;
       w.step = p.causal;
       w.token = at.r.start + first;
-      w.part = p.cluster ? 1 : w.blk == 0 && w.end == at.nblk ? 0 : w.blk > 0 ? 1 : 2;
+      w.part = p.cluster ? 1 : at.blk == 0 && end == at.nblk ? 0 : at.blk > 0 ? 1 : 2;
       if (w.part == 2) header = {pa_parts(p, share, x, at.nblk), w.rows, at.tile * p.tile_rows, at.r.start, at.g};
     }
     if (lane == 0) {
@@ -902,8 +921,8 @@ __device__ __forceinline__ void pt_lead(const PagedAttnParams& p, PaPlace at, co
     }
     __syncwarp();
     ++queries;
-    x += w.end - w.blk;
-    if (x < share.x1) pa_next<pt_bk(D)>(p, at);
+    x += end - at.blk;
+    if (x < share.x1) pa_next<pt_bk(D)>(p, at, share.extra);
   }
   if (queries > 0) mbar_wait(&bars.q_full, (queries - 1) & 1);
   if (lane == 0 && !p.cluster) reinterpret_cast<PaHeader*>(p.ws)[blockIdx.x] = header;
@@ -1864,10 +1883,11 @@ int tybok_paged_attention(const void* q, int64_t ldq, const void* k_pages, const
   p.wide_out = ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_planes)) & 31) == 0;
   const bool tiles = pa_tile_form(p.ratio, max_tokens);
   p.tile_rows = !tiles ? PR_ROWS : 128 / p.ratio * p.ratio * (D == 128 ? 2 : 1);
-  const double most_tiles = static_cast<double>(tokens) * p.ratio / p.tile_rows + B, most_blocks = static_cast<double>(table_width) * page_size / 64 + 1;
+  const double most_tiles = static_cast<double>(tokens) * p.ratio / p.tile_rows + B, most_blocks = static_cast<double>(table_width) * page_size / 64 + 8;
   if (most_tiles * G * most_blocks > 4e9) return host::fail(TYBOK_ERR_ARG, "paged_attention: more than 2^32 key blocks could fall to one call");
   p.tile_tokens = p.tile_rows % p.ratio == 0 ? p.tile_rows / p.ratio : 0;
   p.join_blocks = tiles ? (D == 128 ? 3 : 9) : 4;
+  p.tile_blocks = !tiles ? 0 : D == 128 ? 2 : 5;
   CUtensorMap tm_q, tm_k, tm_v;
   if (tiles) {
     const uint64_t dims[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(p.ratio), static_cast<uint64_t>(G), static_cast<uint64_t>(tokens)};
