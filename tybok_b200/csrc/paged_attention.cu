@@ -172,7 +172,8 @@ struct PaGroup {      // 32 requests
 };
 struct PaLine {
   uint32_t places, tiles;
-  int longest, extra;                     // blocks of the longest tile
+  int extra;
+  bool whole;                             // no tile is to have two CTAs
   uint32_t sums[PA_MAX_REQUESTS / 1024];  // places of group 32 i + lane
   PaGroup last;
 };
@@ -219,12 +220,13 @@ template <int BK>
 __device__ __forceinline__ PaLine pa_line(const PagedAttnParams& p) {
   const int lane = threadIdx.x & 31;
   PaLine line{};
+  int longest = 0;  // tile, in blocks
   uint32_t tiles[PA_MAX_REQUESTS / 1024] = {}, all_tiles = 0;  // up to this lane's request in the last group
 #pragma unroll 1
   for (int k = 0; 32 * k < p.B; ++k) {
     line.last = pa_group<BK>(p, k, 0);
     all_tiles = pa_scan(static_cast<uint32_t>(line.last.tiles) * p.G);
-    if (!p.cluster && line.last.tiles > 0) line.longest = max(line.longest, pa_blocks<BK>(p, line.last.r, line.last.tiles - 1));
+    if (!p.cluster && line.last.tiles > 0) longest = max(longest, pa_blocks<BK>(p, line.last.r, line.last.tiles - 1));
     const uint32_t sum = __shfl_sync(0xffffffffu, line.last.sum, 31), count = __shfl_sync(0xffffffffu, all_tiles, 31);
 #pragma unroll
     for (int i = 0; i < PA_MAX_REQUESTS / 1024; ++i)
@@ -232,9 +234,13 @@ __device__ __forceinline__ PaLine pa_line(const PagedAttnParams& p) {
     line.places += sum;
     line.tiles += count;
   }
-  line.longest = __reduce_max_sync(0xffffffffu, line.longest);
-  if (p.cluster || line.places < p.tile_blocks * gridDim.x) return line;
-  line.extra = p.tile_blocks;
+  if (p.cluster) return line;
+  const uint32_t ctas = gridDim.x;
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (line.places >= p.tile_blocks * ctas) line.extra = p.tile_blocks;
+  const uint32_t per = (line.places + line.tiles * line.extra + ctas - 1) / ctas;
+  line.whole = static_cast<float>((line.tiles + ctas - 1) / ctas) * (longest + line.extra) <= static_cast<float>(per + line.extra + p.join_blocks);
+  if (line.whole) line.extra = 0;  // about equal tiles
   line.places += line.tiles * line.extra;
 #pragma unroll
   for (int i = 0; i < PA_MAX_REQUESTS / 1024; ++i) line.sums[i] += tiles[i] * line.extra;
@@ -324,8 +330,8 @@ __device__ __forceinline__ void pa_next(const PagedAttnParams& p, PaPlace& at, i
 }
 
 // A CTA's share [x0, x1) of the line: equal numbers of places, borders moved to the edge of a tile that lies near (and from a tile's
-// leading places to its beginning).  With `whole` every border moves to the nearest edge, so no tile has two CTAs: where the
-// rounds of whole tiles take no longer than an even share and the joining of its parts.
+// leading places to its beginning).  With `whole` every border moves to the nearest edge: where the rounds of the longest tile take
+// no longer than an even share, the second beginning that it brings and the joining of its parts.
 struct PaShare {
   uint32_t per, x0, x1;
   int extra;
@@ -355,7 +361,7 @@ __device__ PaShare pa_share(const PagedAttnParams& p, PaPlace& first) {
   }
   const uint32_t ctas = gridDim.x;
   sh.per = (line.places + ctas - 1) / ctas;
-  sh.whole = static_cast<float>((line.tiles + ctas - 1) / ctas) * (line.longest + line.extra) <= static_cast<float>(sh.per + p.join_blocks);
+  sh.whole = line.whole;
   PaPlace next{};
   uint32_t border[2];
 #pragma unroll 1
