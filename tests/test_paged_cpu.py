@@ -82,7 +82,7 @@ def test_plan_refuses(over, in_place):
     dict(k_pages=_bf(P, G, D, PAGE).transpose(2, 3), v_pages=_bf(P, G, D, PAGE).transpose(2, 3)),
     dict(k_pages=_bf(1, G, PAGE, D).expand(P, G, PAGE, D)),  # pages on top of one another
     dict(k_pages=_bf(P * G * PAGE * D + 8)[4:-4].view(P, G, PAGE, D)),  # not aligned
-    dict(norm_q=torch.ones(D - 1)), dict(norm_k=_bf(D)),
+    dict(norm_q=torch.ones(D - 1)), dict(norm_k=_bf(D)), dict(cos=torch.zeros(64, D + 8), sin=torch.zeros(64, D + 8)),
 ])
 def test_store_refuses(over):
     with pytest.raises((TypeError, ValueError)):
@@ -94,6 +94,7 @@ def test_store_refuses(over):
     dict(k_pages=_bf(P, G, PAGE, D).float()), dict(v_pages=_bf(P + 1, G, PAGE, D)), dict(block_table=_i(B - 1, W)),
     dict(block_table=_i(W, B).t()), dict(block_table=_i(B, W).long()), dict(cu_tokens=_i(B)), dict(cu_tokens=_i(B + 1).long()),
     dict(key_lens=_i(B + 1)), dict(key_lens=_i(0), cu_tokens=_i(1), block_table=_i(0, W)), dict(max_tokens=0), dict(out_bf16=False),
+    dict(k_pages=_bf(1, G, PAGE, D).expand(P, G, PAGE, D)), dict(v_pages=_bf(P, 1, PAGE, D).expand(P, G, PAGE, D)),
 ])
 def test_attention_refuses(over):
     with pytest.raises((TypeError, ValueError)):
@@ -135,6 +136,8 @@ def _c(entry, **over):
     ("tybok_paged_attention", dict(ldq=H * D + 4), "aligned"), ("tybok_paged_attention", dict(v=ctypes.c_void_p(24)), "aligned"),
     ("tybok_paged_attention", dict(shift=61), "exponent"), ("tybok_paged_attention", dict(ws=None), "workspace"),
     ("tybok_paged_attention", dict(bytes=16), "workspace"), ("tybok_paged_attention", dict(tokens=1 << 30), "31 bits"),
+    ("tybok_paged_attention", dict(width=1 << 27), "31 bits"), ("tybok_paged_attention", dict(ks=(ctypes.c_int64 * 3)(0, PAGE * D, D)), "positive"),
+    ("tybok_head_norm_rope_store", dict(vs=(ctypes.c_int64 * 3)(G * PAGE * D, 0, D)), "positive"),
 ])
 def test_c_entry_points_refuse(entry, over, says):
     rc, message = _c(entry, **over)

@@ -246,3 +246,26 @@ def test_outputs_that_are_only_16_byte_aligned(lens, new, h, g, d):
     assert torch.equal(out[8 : 8 + n].view_as(want), want) and bool((out[:8] == 7).all()) and bool((out[8 + n :] == 7).all())
     assert torch.equal(out_planes[16 : 16 + 3 * n], planes.view(torch.uint8).reshape(-1))
     assert bool((out_planes[:16] == 9).all()) and bool((out_planes[16 + 3 * n :] == 9).all())
+
+
+def test_plan_refuses_lengths_beyond_31_bits():
+    from tybok_b200 import ops
+
+    table, free = torch.zeros(1, 2050, dtype=torch.int32, device="cuda"), _i32([0, 1, 2, 3])
+    plan = ops.page_plan(_i32([2**31 - 100]), _i32([200]), table, free, _i32([4]), tokens=200, page_size=1 << 20)
+    assert plan.missing.item() == -1 and plan.key_lens.item() == 2**31 - 100 and bool((plan.slots == -1).all())
+
+
+@pytest.mark.parametrize("h,g,d", [(8, 1, 256), (8, 2, 128), (1, 1, 128)])
+def test_requests_that_claim_the_same_tokens_are_reported(h, g, d):
+    """Bounds that go back and forth: the status word says so, rows outside the output are never touched."""
+    from tybok_b200 import ops
+
+    q, kp, vp, table, _, _ = _attention_inputs([60] * 6, [40] * 6, h, g, d, 16, seed=12)
+    out = ops.paged_attention(q, kp, vp, table, _i32([0, 240, 0, 240, 0, 240, 0]), _i32([60] * 6), scale=0.1, causal=False)[0]
+    torch.cuda.synchronize()
+    with pytest.raises(ops._lib.TybokError, match="out of range"):
+        ops.check_status()
+    assert out.shape == q.shape
+    y, _ = _check_attention((q, kp, vp, table, _i32([0, 40, 80, 120, 160, 200, 240]), _i32([60] * 6)), 0.1, False)  # and the next call is right
+    assert y.shape == q.shape

@@ -67,19 +67,20 @@ static Plan page_plan(const Tensor& lens, const Tensor& fresh, const Tensor& tab
 }
 
 // A pool of pages [P, G, page, D]: any strides that the kernels' 16-byte accesses take.
-static void need_pool(const Tensor& t, const char* what, const char* name, bool written) {
+static void need_pool(const Tensor& t, const char* what, const char* name) {
   const std::string who = std::string(what) + ": " + name;
   if (!is_bf16(t) || t.dim() != 4 || t.numel() == 0) type_error(who + " must be bf16 [pages, kv heads, page size, head dim]");
   bool ok = t.stride(3) == 1 && !(reinterpret_cast<uintptr_t>(t.data_ptr()) & 15);
-  for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) % 8 == 0 && (t.stride(i) != 0 || !written || t.size(i) == 1);
-  if (!ok) type_error(who + " must have unit stride along the head, other strides multiples of 8 elements and a 16-byte aligned start");
+  for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) % 8 == 0 && (t.stride(i) > 0 || t.size(i) == 1);
+  if (!ok) type_error(who + " must have unit stride along the head, other strides positive multiples of 8 elements and a 16-byte aligned start");
+  if (t.size(0) > 0x7fffffff || t.size(2) > 0x7fffffff) value_error(who + ": pages and their size must be 31-bit numbers");
 }
 
 static Tensor head_norm_rope_store(const Tensor& qkv, const Tensor& pos, const Tensor& slots, const Tensor& cos, const Tensor& sin, const Tensor& kp,
                                    const Tensor& vp, int64_t heads, const OptTensor& norm_q, const OptTensor& norm_k, double eps, bool paired) {
   const char* what = "head_norm_rope_store";
-  need_pool(kp, what, "k_pages", true);
-  need_pool(vp, what, "v_pages", true);
+  need_pool(kp, what, "k_pages");
+  need_pool(vp, what, "v_pages");
   if (kp.sizes() != vp.sizes()) value_error("head_norm_rope_store: key and value pages differ in shape");
   const int64_t g = kp.size(1), page = kp.size(2), d = kp.size(3);
   if (!is_bf16(qkv) || qkv.dim() != 2) type_error("head_norm_rope_store: qkv must be bf16 [tokens, (H + 2G) * D]");
@@ -90,6 +91,7 @@ static Tensor head_norm_rope_store(const Tensor& qkv, const Tensor& pos, const T
   if (cos.scalar_type() != at::kFloat || cos.dim() != 2 || !cos.is_contiguous() || sin.scalar_type() != at::kFloat || !sin.is_contiguous() ||
       sin.sizes() != cos.sizes())
     type_error("head_norm_rope_store: cos and sin must be contiguous fp32 [positions, rotated channels / 2]");
+  if (t > 0x7fffffff || cos.size(0) > 0x7fffffff || cos.size(1) > d) value_error("head_norm_rope_store: sizes must be 31-bit numbers, rotated channels at most the head's");
   for (const Tensor* w : {opt(norm_q), opt(norm_k)})
     if (w && !is_vector(*w, at::kFloat, d)) type_error("head_norm_rope_store: norm weights must be contiguous fp32 [head dim]");
   same_device(qkv.device(), what, {&pos, &slots, &cos, &sin, &kp, &vp, opt(norm_q), opt(norm_k)});
@@ -111,8 +113,8 @@ static std::tuple<Tensor, Tensor> paged_attention(const Tensor& q, const Tensor&
                                                   const Tensor& lens, double scale, bool causal, std::optional<int64_t> max_tokens, bool out_bf16,
                                                   bool out_planes, int out_shift) {
   const char* what = "paged_attention";
-  need_pool(kp, what, "k_pages", false);
-  need_pool(vp, what, "v_pages", false);
+  need_pool(kp, what, "k_pages");
+  need_pool(vp, what, "v_pages");
   if (kp.sizes() != vp.sizes()) value_error("paged_attention: key and value pages differ in shape");
   const int64_t g = kp.size(1), page = kp.size(2), d = kp.size(3), b = lens.numel();
   if (!is_bf16(q) || q.dim() != 2) type_error("paged_attention: q must be bf16 [tokens, H * D]");
@@ -123,6 +125,7 @@ static std::tuple<Tensor, Tensor> paged_attention(const Tensor& q, const Tensor&
   need_ints(cu, b + 1, what, "cu_tokens");
   if (table.scalar_type() != at::kInt || table.dim() != 2 || table.size(0) != b || table.size(1) < 1 || table.stride(1) != 1)
     type_error("paged_attention: block_table must be int32 [B, width] with unit inner stride");
+  if (b > 0x7fffffff || t > 0x7fffffff || table.size(1) > 0x7fffffff) value_error("paged_attention: sizes must be 31-bit numbers");
   if (!out_bf16 && !out_planes) value_error("at least one of out_bf16 / out_planes must be set");
   if (max_tokens && *max_tokens < 1) value_error("paged_attention: max_tokens must be positive");
   same_device(q.device(), what, {&kp, &vp, &table, &cu, &lens});

@@ -7,7 +7,8 @@
 // their order.  Queries of the same key head are rows of the same product (row = token * H / G + head).
 //
 // Where the tiles are few and the caches short, a cluster of CTAs takes each tile instead and joins its parts over distributed
-// shared memory: no second kernel, no trip through global memory.
+// shared memory: no second kernel, no trip through global memory (3 requests of 10 keys, 8 heads of 256: 7.6 us against 8.6; 8 requests of
+// 50 tokens over up to 970 keys: 14.7 against 21.8).
 //
 // Algorithmic bytes: Q and O once, K and V of a request's keys once per row tile (L2 serves the tiles after the first).
 // Flops: 4 * D * H per visible (query, key) pair.
@@ -279,10 +280,10 @@ __device__ __forceinline__ PaPlace pa_locate(const PagedAttnParams& p, const PaL
   const uint32_t per_head = __shfl_sync(0xffffffffu, g.cost, src);
   x -= __shfl_sync(0xffffffffu, g.sum, src) - per_head * p.G;
   PaPlace at{};
-  at.b = 32 * k + src;
+  at.b = min(32 * k + src, p.B - 1);  // (only tokens counted many times over could lead beyond the line)
   at.r = {__shfl_sync(0xffffffffu, g.r.start, src), __shfl_sync(0xffffffffu, g.r.n, src), __shfl_sync(0xffffffffu, g.r.len, src)};
   at.tiles = __shfl_sync(0xffffffffu, g.tiles, src);
-  at.g = p.G == 1 ? 0 : static_cast<int>(x / per_head);
+  at.g = p.G == 1 ? 0 : static_cast<int>(min(x / max(per_head, 1u), p.G - 1u));
   x -= at.g * per_head;
   if (p.cluster) {
     at.tile = static_cast<int>(x);
@@ -319,7 +320,7 @@ __device__ __forceinline__ void pa_next(const PagedAttnParams& p, PaPlace& at, i
     if (++at.g == p.G) {
       at.g = 0;
       do {
-        ++at.b;
+        at.b = min(at.b + 1, p.B - 1);
         at.r = pa_request(p, at.b);
       } while (at.r.n == 0 && at.b + 1 < p.B);
       at.tiles = pa_tiles(p, at.r.n);
@@ -682,20 +683,25 @@ __global__ void __launch_bounds__(PR_THREADS, pr_ctas(D)) paged_rows_kernel(cons
 }
 
 // ------------------------------------------------------------------------------------------------ tile forms
-// Many rows per key head: 128-row tiles on the fifth-generation tensor cores.  Four control warps (the CTA's share, keys and values,
-// one or two that issue the products) and two groups of four softmax warps with one query row per thread and tensor-memory
+// Many rows per key head: 128-row tiles on the fifth-generation tensor cores.  Four control warps (keys, products, values, and the
+// CTA's share with the queries) and two groups of four softmax warps with one query row per thread and tensor-memory
 // lane.  The warp that walks the CTA's share tells the others, a few tiles ahead; rings and barriers run on from tile to tile, so
 // the next tile's queries, keys and first scores are on their way while this one's output is written.
 //   S = Q K^T into tensor memory, P = 2^(S c - m) in bf16 over it (m: a reference that moves only when a block's maximum exceeds
 //   it by more than 2^8, then the row of O is rescaled), O += P V with P read from tensor memory.
-//   head_dim 128 (paged_pair_kernel): two tiles of 128 rows share every block of 128 keys, a group of softmax warps and a warp that
-//            issues products each (issuing costs 20 to 50 clocks an instruction and about 100 a wait: one warp for both tiles
-//            set the pace); queries in shared memory.  Tensor memory: S / P and O of both tiles, 128 columns each; a tile's
-//            S(j+1) follows its PV(j).  The tiles take turns: one's products run under the other's exponentials.
+//   head_dim 128 (paged_pair_kernel): two tiles of 128 rows share every block of 128 keys, a group of softmax warps each; queries in
+//            shared memory.  Tensor memory: S / P and O of both tiles, 128 columns each; a tile's S(j+1) follows its PV(j).
+//            One warp issues the products of both, so the tiles take turns: one's products run under the other's exponentials
+//            (a warp for each fell into step with the other: 562 to 600 us against 530 on 2 requests of 2048 tokens over
+//            8250 keys; blocks of 64 keys with scores in two buffers 597).  Bound by the exponentials (2048 of the special-function unit's
+//            clocks a block), the products (2048) and the hand-overs between them: 3450 clocks a block.
 //   head_dim 256 (paged_wide_kernel): O of one tile takes half of the tensor memory.  The groups take every other block of 64 keys, with a
 //            score buffer each: PV(j), S(j+2).  The queries are in tensor memory too: as a shared-memory operand their 64 KB
 //            would be read again for every 64 keys, and with the keys, the values and what the copies write, shared
-//            memory (128 bytes a clock) would set the pace (1790 clk a block).
+//            memory (128 bytes a clock) would set the pace (1790 clocks a block, and 1570 so, of which 1024 are products).
+// Measured on a B200: 32 heads on 8 key heads of 128, 2 requests of 2048 new tokens over 8250 keys each, causal, 425 us once and
+// 470 to 490 back to back under the power cap, 1.0 to 1.1 PF/s; 16 + 16 heads of 128, 19 requests from one token to 700 over up to 5000
+// keys 56 us; 8 heads on 1 of 256: 8 requests of 50 tokens over up to 970 keys 14.7 us, 5 of 402 to 627 tokens over themselves 30.5.
 // A page is one box of the tensor map and 64 channels (or a block's rows of a larger page); lanes of the copying warp issue one
 // box each.  Page numbers out of range read as zero through the map's bounds.
 // Values behind a request's last key are zeroed in shared memory before their product (their weights are zero, but what lies
@@ -1828,7 +1834,8 @@ static int pa_set_attributes() {
 // Tensor map of a pool [P][G][page][D]: boxes of 64 channels and one page's rows (or a block's).
 static int pa_pool_map(CUtensorMap* map, const void* base, const int64_t* strides, int P, int G, int page, int D) {
   const uint64_t dims[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(page), static_cast<uint64_t>(G), static_cast<uint64_t>(P)};
-  const uint64_t pitch[3] = {static_cast<uint64_t>(strides[2]) * 2, static_cast<uint64_t>(strides[1]) * 2, static_cast<uint64_t>(strides[0]) * 2};
+  auto bytes = [&](int i, int extent) { return static_cast<uint64_t>(extent > 1 ? strides[i] : D) * 2; };  // (of an extent of one it does not matter)
+  const uint64_t pitch[3] = {bytes(2, page), bytes(1, G), bytes(0, P)};
   const uint32_t box[4] = {64, static_cast<uint32_t>(std::min(page, pt_bk(D))), 1, 1};
   return host::tensor_map_4d(map, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dims, pitch, box);
 }
@@ -1857,6 +1864,10 @@ int tybok_paged_attention(const void* q, int64_t ldq, const void* k_pages, const
   if (tokens <= 0 || B <= 0 || B > PA_MAX_REQUESTS || H <= 0 || G <= 0 || H % G != 0 || num_pages <= 0 || table_width <= 0 || max_tokens <= 0)
     return host::fail(TYBOK_ERR_ARG, "paged_attention: bad shape (1 to 2048 requests, H % G == 0, pool and table not empty)");
   if (static_cast<long long>(tokens) * (H / G) > 0x7fffffffll) return host::fail(TYBOK_ERR_ARG, "paged_attention: query rows must fit 31 bits");
+  if (static_cast<long long>(table_width) * page_size > 0x7fffff00ll) return host::fail(TYBOK_ERR_ARG, "paged_attention: a request's keys must fit 31 bits");
+  const int extents[3] = {num_pages, G, page_size};
+  for (int i = 0; i < 3; ++i)
+    if (extents[i] > 1 && (k_strides[i] <= 0 || v_strides[i] <= 0)) return host::fail(TYBOK_ERR_ARG, "paged_attention: strides of the pools must be positive");
   const uintptr_t bits = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages) |
                          reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_planes);
   int64_t strides = ldq;
