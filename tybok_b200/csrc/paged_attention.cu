@@ -1047,7 +1047,7 @@ __device__ __forceinline__ void pt_store32(const PagedAttnParams& p, long long a
   }
 }
 // A partial tile in the workspace: four channels of 128 rows side by side, so that a warp's rows are one run: float4 number
-// (64-column order) [column / 4][row].
+// [column / 4][row].
 __device__ __forceinline__ void pt_part32(float4* part, int column, int row, const uint32_t (&o)[32]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e)
