@@ -22,8 +22,8 @@ namespace tb {
 // Every CTA makes the sums itself (a few thousand lengths out of L2), so CTAs share nothing: functional calls spread over as
 // many as the copies and tokens need, without a barrier; calls in place run as one cluster that meets once, between
 // reading the old state and writing the new.
-// Bound by latency: the launch, the lengths, the scan, one table entry, the stores.  In a graph: 48 requests with a token each 5.2 us, 7 prompts
-// 3.9, 2048 requests with 45,000 tokens 8.8 (2.5 MB).
+// Bound by latency: the launch, the lengths, the scan, one table entry, the stores.  In a graph: 48 requests with a token each 3.8 us, 7 prompts
+// 2.95, 2048 requests with 45,000 tokens 6.0 (2.5 MB).
 struct PlanParams {
   const int* lens;
   const int* fresh;           // new tokens per request
@@ -161,12 +161,15 @@ __global__ void __launch_bounds__(1024) page_plan_kernel(const PlanParams p) {
     if (p.in_place) return __ldcg(p.stack_out + i);
     return i < count ? p.stack[i] : back_page(i - count);
   };
-  for (int x = g0; x < nmore; x += gn) {
+  // The rest begins with other CTAs than the copies: each part is a chain of its own (48 requests 3.7 us against 5.1, 2048 requests 6.0 against 8.8).
+  const int half = gridDim.x >> 1, g1 = (blockIdx.x < half ? blockIdx.x + gridDim.x - half : blockIdx.x - half) * n + tid;
+  const int g2 = (gridDim.x - 1 - blockIdx.x) * n + tid;
+  for (int x = g1; x < nmore; x += gn) {
     const int b = plan_find(more, p.B, x);
     p.table_out[static_cast<long long>(b) * p.W + plan_pages(base[b], p.page_shift) + x - more[b]] = taken(x);
   }
   const int page = 1 << p.page_shift, real = ok ? cu[p.B] : 0;
-  for (int t = g0; t < p.T; t += gn) {
+  for (int t = g2; t < p.T; t += gn) {
     int at = 0, slot = -1;
     if (t < real) {
       const int b = plan_find(cu, p.B, t);
@@ -439,10 +442,11 @@ int tybok_page_plan(const int* key_lens, const int* new_lens, const void* finish
   p.cu = cu_tokens; p.pos = pos; p.slots = slots; p.missing = missing;
   p.B = B; p.W = table_width; p.P = num_pages; p.T = tokens; p.page_shift = shift; p.in_place = same == 4;
   p.pdl = host::pdl_enabled() ? 1 : 0;
-  // entries to copy and write, two a thread: every CTA pays the whole scan, but side by side
+  // Two threads for an entry to copy or write: every CTA pays the whole scan, but side by side, and the chains of the parts fall to different ones (7
+  // prompts 2.95 us, 4.0 with two entries a thread; more than a CTA per SM costs 2048 requests 2.4 us).  In place, where one cluster meets, two entries a thread.
   const long long work = tokens + (p.in_place ? 0ll : num_pages + static_cast<long long>(B) * table_width);
   const int threads = B <= 256 ? 256 : B <= 1024 ? 512 : 1024, most = p.in_place ? 8 : host::sm_count();
-  const int ctas = static_cast<int>(std::min<long long>(most, std::max<long long>(1, work / (2 * threads))));
+  const int ctas = static_cast<int>(std::min<long long>(most, std::max<long long>(1, p.in_place ? work / (2 * threads) : 2 * work / threads)));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(p.in_place && ctas > 1 ? 8 : ctas);
   cfg.blockDim = dim3(threads);
