@@ -44,6 +44,8 @@ struct PagedAttnParams {
   long long ld_out;  // H * D
   float plane_scale;
   int T, B, H, G, ratio, P, W, page_shift, causal;
+  uint32_t ratio_mul;
+  int ratio_shift;
   int tile_rows;     // query rows (token, head of the group) of a tile, at most those of the form
   int tile_tokens;   // tokens of a tile where it holds whole ones, else 0
   int wide_out;      // the outputs are 32-byte aligned
@@ -58,6 +60,12 @@ struct PagedAttnParams {
   int* status;
   int pdl;
 };
+
+// n / ratio for 0 <= n < 2^31, by a product with ratio_mul = ceil(2^(31 + bits) / ratio), bits = ceil(log2(ratio)): exact for 31 bits, and no
+// division (150 clocks and more) on the way to the first keys.
+__device__ __forceinline__ int pa_token(const PagedAttnParams& p, int row) {
+  return p.ratio == 1 ? row : static_cast<int>(__umulhi(static_cast<uint32_t>(row), p.ratio_mul) >> p.ratio_shift);
+}
 
 // What a CTA's share needs to know of one request, out of range values brought back into range.
 struct PaRequest {
@@ -78,7 +86,7 @@ __device__ __forceinline__ bool pa_in_range(const PagedAttnParams& p, int b) {
 // Keys that the rows before `row_end` of a request see: those of the last of them.
 __device__ __forceinline__ int pa_seen(const PagedAttnParams& p, const PaRequest& r, int row_end) {
   if (!p.causal) return r.len;
-  return max(0, r.len - r.n + (row_end - 1) / p.ratio + 1);
+  return max(0, r.len - r.n + (row_end > 0 ? pa_token(p, row_end - 1) : -1) + 1);
 }
 // Key blocks of a row tile; a tile that sees no key is one block of work all the same (its output is zero).
 template <int BK>
@@ -444,7 +452,7 @@ __global__ void __launch_bounds__(PR_THREADS, pr_ctas(D)) paged_rows_kernel(cons
     const int end = static_cast<int>(min(static_cast<uint32_t>(at.nblk), at.blk + (x1 - x)));
     const int rows = at.r.n * p.ratio;
     const int seen = pa_seen(p, at.r, min(rows, (at.tile + 1) * PR_ROWS));                    // by any row
-    const int seen_all = p.causal ? max(0, at.r.len - at.r.n + at.tile * PR_ROWS / p.ratio + 1) : at.r.len;  // by every row
+    const int seen_all = p.causal ? max(0, at.r.len - at.r.n + pa_token(p, at.tile * PR_ROWS) + 1) : at.r.len;  // by every row
     uint32_t in = 0, out = 0;  // ring slots
     auto fetch = [&](int j) {  // this warp's keys of block j
       const uint32_t slot = ring + in * STAGE;
@@ -476,7 +484,7 @@ __global__ void __launch_bounds__(PR_THREADS, pr_ctas(D)) paged_rows_kernel(cons
         // this thread's two rows of the tile: queries as operand fragments, keys they see
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int row = at.tile * PR_ROWS + h * 8 + (lane >> 2), token = row / p.ratio;
+          const int row = at.tile * PR_ROWS + h * 8 + (lane >> 2), token = pa_token(p, row);
           const bool live = row < rows;
           limit[h] = !live ? 0 : p.causal ? max(0, at.r.len - at.r.n + token + 1) : at.r.len;
           const __nv_bfloat16* src = p.q + (at.r.start + token) * p.ldq + static_cast<long long>(at.g * p.ratio + row - token * p.ratio) * D + (lane & 3) * 2;
@@ -614,7 +622,7 @@ __global__ void __launch_bounds__(PR_THREADS, pr_ctas(D)) paged_rows_kernel(cons
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= inv;
-        const int token = grow / p.ratio;
+        const int token = pa_token(p, grow);
         pa_store8(p, (at.r.start + token) * p.ld_out + static_cast<long long>(at.g * p.ratio + grow - token * p.ratio) * D + c, v);
       } else if (p.cluster) {
         const int owner = row / each, at_owner = rank * each + row % each;
@@ -677,7 +685,7 @@ __global__ void __launch_bounds__(PR_THREADS, pr_ctas(D)) paged_rows_kernel(cons
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] *= inv;
-    const int token = grow / p.ratio;
+    const int token = pa_token(p, grow);
     pa_store8(p, (at.r.start + token) * p.ld_out + static_cast<long long>(at.g * p.ratio + grow - token * p.ratio) * D + c, v);
   }
 }
@@ -1259,7 +1267,7 @@ __device__ __forceinline__ void pt_join(const PagedAttnParams& p, const PtBars& 
         o[4 * e + 3] = __float_as_uint(__uint_as_float(o[4 * e + 3]) + f * a.w);
       }
     }
-    const int ahead = local / p.ratio;
+    const int ahead = pa_token(p, local);
     pt_store32(p, static_cast<long long>(bars.item.token + ahead) * p.ld_out + static_cast<long long>(bars.item.g * p.ratio + local - ahead * p.ratio) * D + c * 32, o,
                sum == 0.f ? 0.f : 1.f / sum);
   }
@@ -1369,7 +1377,7 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
     const uint32_t t_s = tmem + t * 128 + lane_addr, t_o = tmem + 256 + t * 128 + lane_addr;
     const uint64_t c2 = pt_pair(p.abs_scale_log2e, p.abs_scale_log2e);
-    const int local = t * half + row, ahead = local / p.ratio;  // row of the piece; its token's number in it
+    const int local = t * half + row, ahead = pa_token(p, local);  // row of the piece; its token's number in it
     pa_check(p, tid - 128, 256);
     pa_zero_rows<D>(p, tid - 128, 256);
     uint32_t n = 0, i = 0;  // tiles and blocks of this group
@@ -1555,7 +1563,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
     const uint32_t t_o = tmem + 256 + lane_addr, t_s = tmem + grp * 64 + lane_addr;
     const uint64_t c2 = pt_pair(p.abs_scale_log2e, p.abs_scale_log2e);
-    const int ahead = row / p.ratio;  // number of the row's token in the tile
+    const int ahead = pa_token(p, row);  // number of the row's token in the tile
     uint32_t i = 0;                   // blocks so far (of both groups)
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -1702,7 +1710,7 @@ __global__ void __launch_bounds__(128) paged_join_tile_kernel(const PagedAttnPar
   const PaHeader h = reinterpret_cast<const PaHeader*>(p.ws)[blockIdx.x];
   if (h.parts == 0) return;
   constexpr int ROWS = pt_rows(D), COLS = D / 32;  // grid.y = 32 columns of 128 rows
-  const int t = blockIdx.y / COLS, c = blockIdx.y % COLS, row = threadIdx.x, half = 128 / p.ratio * p.ratio, local = t * half + row;
+  const int t = blockIdx.y / COLS, c = blockIdx.y % COLS, row = threadIdx.x, half = p.tile_rows / (pt_rows(D) / 128), local = t * half + row;
   if (row >= half || local >= h.rows) return;
   const uint8_t* parts = p.ws + pa_header_bytes(ctas);
   auto part = [&](int i) {  // the i-th part of the tile
@@ -1731,7 +1739,7 @@ __global__ void __launch_bounds__(128) paged_join_tile_kernel(const PagedAttnPar
       o[4 * e + 3] = __float_as_uint(__uint_as_float(o[4 * e + 3]) + f * a[e].w);
     }
   }
-  const int grow = h.first + local, token = grow / p.ratio;
+  const int grow = h.first + local, token = pa_token(p, grow);
   pt_store32(p, static_cast<long long>(h.start + token) * p.ld_out + static_cast<long long>(h.g * p.ratio + grow - token * p.ratio) * D + c * 32, o, sum == 0.f ? 0.f : 1.f / sum);
 }
 
@@ -1769,7 +1777,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnParams p
       }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int grow = h.first + row, token = grow / p.ratio;
+    const int grow = h.first + row, token = pa_token(p, grow);
     const long long at = static_cast<long long>(h.start + token) * p.ld_out + static_cast<long long>(h.g * p.ratio + grow - token * p.ratio) * D;
     float o[8];  // eight channels by one lane: its own, or (four channels per lane) its own and its neighbour's
 #pragma unroll
@@ -1889,6 +1897,10 @@ int tybok_paged_attention(const void* q, int64_t ldq, const void* k_pages, const
   p.ld_out = static_cast<long long>(H) * D; p.plane_scale = ldexpf(1.0f, out_shift);
   p.T = tokens; p.B = B; p.H = H; p.G = G; p.ratio = H / G; p.P = num_pages; p.W = table_width; p.causal = causal;
   for (p.page_shift = 4; (1 << p.page_shift) != page_size;) ++p.page_shift;
+  int ratio_bits = 1;
+  while ((1ll << ratio_bits) < p.ratio) ++ratio_bits;
+  p.ratio_mul = static_cast<uint32_t>(((1ull << (31 + ratio_bits)) + p.ratio - 1) / p.ratio);  // (not used for a ratio of one)
+  p.ratio_shift = ratio_bits - 1;
   p.scale_log2e = scale * 1.4426950408889634f;
   // the tile forms want a scale above zero (at zero: one that no score brings above 2^-22)
   p.abs_scale_log2e = fabsf(p.scale_log2e);
