@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(PR_THREADS, pr_ctas(D)) paged_rows_kernel(cons
   PaHeader header{};
   // cluster: [CTA][row of this CTA's share][D], then the references and the sums, as the CTAs send them
   float* parts = reinterpret_cast<float*>(pr_shared + pr_ring(D));
-  const int each = p.cluster ? PR_ROWS / p.cluster : PR_ROWS, rank = p.cluster ? static_cast<int>(cluster_ctarank()) : 0;
+  const int each = p.cluster ? PR_ROWS / p.cluster : PR_ROWS, each_bits = __ffs(each) - 1, rank = p.cluster ? static_cast<int>(cluster_ctarank()) : 0;
   bool tidied = false;
   auto tidy = [&] {  // under the first keys' way
     pa_check(p, tid, PR_THREADS);
@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(PR_THREADS, pr_ctas(D)) paged_rows_kernel(cons
         *reinterpret_cast<float2*>(mine + row * D + ((i * 8 + (lane & 3) * 2) ^ ((row & 3) << 3))) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
     }
     __syncthreads();
-    const bool whole_tile = !p.cluster && at.blk == 0 && end == at.nblk;
+    const bool whole_tile = at.blk == 0 && end == at.nblk;
     const int part = at.blk > 0 ? 0 : 1;
     if (p.cluster) cluster_wait_acquire();  // the others are there
     float* po = reinterpret_cast<float*>(p.ws + pa_header_bytes(gridDim.x) + (2ll * blockIdx.x + part) * pa_part_bytes<PR_ROWS, D>());
@@ -625,7 +625,7 @@ __global__ void __launch_bounds__(PR_THREADS, pr_ctas(D)) paged_rows_kernel(cons
         const int token = pa_token(p, grow);
         pa_store8(p, (at.r.start + token) * p.ld_out + static_cast<long long>(at.g * p.ratio + grow - token * p.ratio) * D + c, v);
       } else if (p.cluster) {
-        const int owner = row / each, at_owner = rank * each + row % each;
+        const int owner = row >> each_bits, at_owner = rank * each + (row & (each - 1));
         const uint32_t to = dsmem_addr(smem_u32(parts + at_owner * D + c), owner);
         pa_send4(to, make_float4(v[0], v[1], v[2], v[3]));
         pa_send4(to + 16, make_float4(v[4], v[5], v[6], v[7]));
@@ -654,10 +654,12 @@ __global__ void __launch_bounds__(PR_THREADS, pr_ctas(D)) paged_rows_kernel(cons
     if (tid == 0) reinterpret_cast<PaHeader*>(p.ws)[blockIdx.x] = header;
     return;
   }
+  const bool alone = share.per > 0 && share.per >= static_cast<uint32_t>(at.nblk);  // one CTA of the cluster has had all of the tile
   if (x == x1) {  // a CTA without blocks has nothing to add
     cluster_wait_acquire();
-    if (share.per > 0 && tid < PR_ROWS) pa_send(parts + PR_ROWS * D + rank * each + tid % each, tid / each, -INFINITY);
+    if (share.per > 0 && !alone && tid < PR_ROWS) pa_send(parts + PR_ROWS * D + rank * each + (tid & (each - 1)), tid >> each_bits, -INFINITY);
   }
+  if (alone) return;
   __syncwarp();
   cluster_sync_all();  // every part has arrived
   if (share.per == 0) return;  // no tile for the whole cluster
@@ -1218,7 +1220,7 @@ __device__ __forceinline__ void pt_meet() {
 // chunks [c0, c1) of 32 columns of tile t's `row`; m = -INFINITY: no part of it here
 template <int D>
 __device__ __forceinline__ void pt_send(const PagedAttnParams& p, PtBars& bars, float4* parts, uint32_t t_o, int t, int row, int c0, int c1, bool live, bool mine, float m, float l) {
-  const int each = pt_rows(D) / p.cluster, at = t * 128 + row, owner = at / each, here = at - owner * each, rank = cluster_ctarank();
+  const int each = pt_rows(D) / p.cluster, at = t * 128 + row, owner = at >> (__ffs(each) - 1), here = at & (each - 1), rank = cluster_ctarank();
   if (c0 == 0) {
     pa_send(&bars.part_m[rank * each + here], owner, mine ? m : -INFINITY);
     pa_send(&bars.part_l[rank * each + here], owner, l);
@@ -1242,7 +1244,7 @@ __device__ __forceinline__ void pt_join(const PagedAttnParams& p, const PtBars& 
   if (bars.item.rows == 0) return;
   const int each = pt_rows(D) / p.cluster, rank = cluster_ctarank(), half = p.tile_rows / (pt_rows(D) / 128);
   for (int i = threadIdx.x - 128; i < each * (D / 32); i += 256) {
-    const int here = i % each, at = rank * each + here, c = i / each, local = (at >> 7) * half + (at & 127);
+    const int here = i & (each - 1), at = rank * each + here, c = i >> (__ffs(each) - 1), local = (at >> 7) * half + (at & 127);
     if ((at & 127) >= half || local >= bars.item.rows) continue;
     float m[8], top = -INFINITY, sum = 0.f;
 #pragma unroll
