@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(HN_THREADS, 8) head_norm_rope_store_kernel(con
   const int lane = threadIdx.x & 31, l = lane % TEAM, sub = lane / TEAM;
   const int c0 = FORM == HN_HALVES ? 4 * l : 8 * l;  // first channel
   const int all = p.H + 2 * p.G;
-  const unsigned w = blockIdx.x * (HN_THREADS / 32) + (threadIdx.x >> 5);
+  const unsigned w = (blockIdx.x * HN_THREADS + threadIdx.x) >> 5;  // (threads fit 32 bits; in another form it costs head_dim 128 a tenth: registers)
   const int t = static_cast<int>(w / p.chunks), h0 = static_cast<int>(w - static_cast<unsigned>(t) * p.chunks) * HEADS + sub;
   if (p.pdl) {
     pdl_launch_dependents();
@@ -515,7 +515,7 @@ int tybok_head_norm_rope_store(const void* src, int64_t ld, const int* pos, cons
   const bool few = static_cast<long long>(tokens) * all < 32768ll * per_load;
   p.chunks = (all + per_load * (few ? 2 : 6) - 1) / (per_load * (few ? 2 : 6));
   const long long ctas = (static_cast<long long>(tokens) * p.chunks * 32 + HN_THREADS - 1) / HN_THREADS;
-  if (ctas > 0x7ffffff) return host::fail(TYBOK_ERR_ARG, "head_norm_rope_store: too many tokens for one launch");
+  if (ctas > 0xffffffffll / HN_THREADS) return host::fail(TYBOK_ERR_ARG, "head_norm_rope_store: too many tokens for one launch");
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(HN_THREADS);
