@@ -7,7 +7,7 @@
 // their order.  Queries of the same key head are rows of the same product (row = token * H / G + head).
 //
 // Where the tiles are few and the caches short, a cluster of CTAs takes each tile instead and joins its parts over distributed
-// shared memory: no second kernel, no trip through global memory (3 requests of 10 keys, 8 heads of 256: 7.6 us against 8.6; 8 requests of
+// shared memory: no second kernel, no trip through global memory (3 requests of 10 keys, 8 heads of 256: 6.8 us against 8.6; 8 requests of
 // 50 tokens over up to 970 keys: 14.7 against 21.8).
 //
 // Algorithmic bytes: Q and O once, K and V of a request's keys once per row tile (L2 serves the tiles after the first).
