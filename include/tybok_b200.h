@@ -333,7 +333,7 @@ int tybok_w8x3_qkv_rope_adarms(const void* u_planes, int u_shift, const float* s
 
 /* ---- paged cache of keys and values --------------------------------------------------------
  * A pool holds num_pages pages [P][G][page_size][D] bf16 in any order of strides with unit stride along D (k_strides /
- * v_strides: elements between pages, heads and rows, multiples of 8; host arrays).  Key j of request b lies in page
+ * v_strides: elements between pages, heads and rows, positive multiples of 8; host arrays).  Key j of request b lies in page
  * block_table[b][j / page_size] at row j % page_size; a slot is page * page_size + row.  page_size is a power of two,
  * 16 at least.  The counterpart of the padded caches [B, G, Lcap, D] that tybok_rope_store and tybok_attention take
  * (tybok/policies/pi05/models/gemma.py:61-125 keeps one per request).

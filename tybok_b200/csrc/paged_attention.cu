@@ -1009,7 +1009,7 @@ __device__ __forceinline__ void pt_clear_tail(uint8_t* block, int len, int j) {
   const int n = (BK - first) * 8;
 #pragma unroll 1
   for (int c = 0; c < D / 64; ++c)
-#pragma unroll 1
+#pragma unroll(D == 256 ? 4 : 1)
     for (int i = threadIdx.x & 31; i < n; i += 32) *reinterpret_cast<uint4*>(block + c * (BK * 128) + first * 128 + i * 16) = make_uint4(0, 0, 0, 0);
   fence_proxy_async();
   __syncwarp();

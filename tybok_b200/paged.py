@@ -22,7 +22,8 @@ from .ops import DEFAULT_SHIFT, PagePlan
 
 class PagedCache:
     """Pools ``k_pages`` / ``v_pages`` ``[layers, pages, kv_heads, page_size, head_dim]`` and the state of ``requests`` rows: ``key_lens``,
-    ``block_table`` (``width`` pages a row; all of them by default), ``free_pages`` and ``free_count``, on ``device``.
+    ``block_table`` (``width`` pages a row, the most that one request may hold; all of them by default, but a width near the truth lets
+    short calls take quicker forms), ``free_pages`` and ``free_count``, on ``device``.
 
     Every request begins with no keys.  All work goes to the current stream of the device; one cache takes one step at a time."""
 
