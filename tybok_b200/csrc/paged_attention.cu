@@ -7,7 +7,7 @@
 // their order.  Queries of the same key head are rows of the same product (row = token * H / G + head).
 //
 // Where the tiles are few and the caches short, a cluster of CTAs takes each tile instead and joins its parts over distributed
-// shared memory: no second kernel, no trip through global memory (3 requests of 10 keys, 8 heads of 256: 6.8 us against 8.6; 8 requests of
+// shared memory: no second kernel, no trip through global memory (3 requests of 10 keys, 8 heads of 256: 6.5 us against 8.6; 8 requests of
 // 50 tokens over up to 970 keys: 14.7 against 21.8).
 //
 // Algorithmic bytes: Q and O once, K and V of a request's keys once per row tile (L2 serves the tiles after the first).
@@ -352,13 +352,24 @@ __device__ __forceinline__ int pa_snap(const PaShare& sh, int blk, int nblk, int
   if (sh.whole || 4 * away <= static_cast<int>(min(sh.per, 4u * join_blocks)) - 4) return up ? nblk : 0;
   return blk <= sh.extra ? 0 : blk;
 }
+// Where share `number` begins, and the place there.
+template <int BK>
+__device__ __forceinline__ uint32_t pa_border(const PagedAttnParams& p, const PaLine& line, const PaShare& sh, unsigned number, PaPlace& next) {
+  const unsigned long long x = static_cast<unsigned long long>(number) * sh.per;
+  if (x >= line.places) return line.places;
+  next = pa_locate<BK>(p, line, static_cast<uint32_t>(x));
+  const int blk = pa_snap(sh, next.blk, next.nblk, p.join_blocks);
+  const uint32_t border = static_cast<uint32_t>(x) - next.blk + blk;
+  next.blk = blk;
+  return border;
+}
 template <int BK>
 __device__ PaShare pa_share(const PagedAttnParams& p, PaPlace& first) {
   const PaLine line = pa_line<BK>(p);
   PaShare sh;
   sh.extra = line.extra;
+  sh.whole = line.whole;
   if (p.cluster) {  // tile number blockIdx.x / cluster; `per` blocks of it to each CTA
-    sh.whole = false;
     sh.per = sh.x0 = sh.x1 = 0;
     const uint32_t x = blockIdx.x / p.cluster, rank = blockIdx.x % p.cluster;
     if (x >= line.tiles) return sh;
@@ -368,25 +379,14 @@ __device__ PaShare pa_share(const PagedAttnParams& p, PaPlace& first) {
     sh.x1 = min(static_cast<uint32_t>(first.nblk) - first.blk, sh.per);
     return sh;
   }
-  const uint32_t ctas = gridDim.x;
-  sh.per = (line.places + ctas - 1) / ctas;
-  sh.whole = line.whole;
-  PaPlace next{};
-  uint32_t border[2];
+  sh.per = (line.places + gridDim.x - 1) / gridDim.x;
 #pragma unroll 1
   for (int i = 1; i >= 0; --i) {
-    const unsigned long long x = static_cast<unsigned long long>(blockIdx.x + i) * sh.per;
-    border[i] = line.places;
-    if (x >= line.places) continue;
-    next = pa_locate<BK>(p, line, static_cast<uint32_t>(x));
-    const int blk = pa_snap(sh, next.blk, next.nblk, p.join_blocks);
-    border[i] = static_cast<uint32_t>(x) - next.blk + blk;
-    next.blk = blk;
+    const uint32_t border = pa_border<BK>(p, line, sh, blockIdx.x + i, first);
+    if (i) sh.x1 = border;
+    else sh.x0 = border;
   }
-  sh.x0 = border[0];
-  sh.x1 = border[1];
-  if (sh.x0 < sh.x1 && next.blk == next.nblk) pa_next<BK>(p, next, sh.extra);
-  first = next;
+  if (sh.x0 < sh.x1 && first.blk == first.nblk) pa_next<BK>(p, first, sh.extra);
   return sh;
 }
 __device__ __forceinline__ void pa_send4(uint32_t to, float4 v) {  // to another CTA of the cluster
