@@ -1,4 +1,6 @@
 // The paged cache: page plan, head norms with rotation and store, attention over pages.
+#include <ATen/cuda/EmptyTensor.h>
+
 #include "native.h"
 
 namespace tbn {
@@ -7,12 +9,17 @@ static void need_ints(const Tensor& t, int64_t n, const char* what, const char* 
   if (!is_vector(t, at::kInt, n)) type_error(std::string(what) + ": " + name + " must be contiguous int32 [" + std::to_string(n) + "]");
 }
 
+// A new tensor on the device of another, without the dispatcher's half a microsecond (the calls here are bound by the host).
+static Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
+}
+
 // Tensors of one allocation, 16-byte aligned pieces of it (an allocation each would cost a call as much as its launch).
 class Pieces {
  public:
   explicit Pieces(const Tensor& like) : like_(like) {}
   void add(int64_t n) { size_ += (n + 3) & ~int64_t(3); }
-  void allocate() { buf_ = at::empty({size_}, like_.options()); }
+  void allocate() { buf_ = new_tensor({size_}, at::kInt, like_); }
   Tensor take(at::IntArrayRef sizes) {
     int64_t n = 1;
     for (const int64_t s : sizes) n *= s;
@@ -98,7 +105,7 @@ static Tensor head_norm_rope_store(const Tensor& qkv, const Tensor& pos, const T
   require_cuda(qkv, what);
   const c10::cuda::CUDAGuard guard(qkv.device());
   const Tensor x = vector_rows_of(qkv);
-  Tensor q = at::empty({t, heads * d}, x.options());
+  Tensor q = new_tensor({t, heads * d}, at::kBFloat16, x);
   if (t == 0) return q;
   const int64_t ks[3] = {kp.stride(0), kp.stride(1), kp.stride(2)}, vs[3] = {vp.stride(0), vp.stride(1), vp.stride(2)};
   check(tybok_head_norm_rope_store(ptr(x), x.stride(0), static_cast<const int*>(pos.data_ptr()), static_cast<const int*>(slots.data_ptr()), f32(cos),
@@ -132,13 +139,12 @@ static std::tuple<Tensor, Tensor> paged_attention(const Tensor& q, const Tensor&
   require_cuda(q, what);
   const c10::cuda::CUDAGuard guard(q.device());
   const Tensor x = vector_rows_of(q);
-  const auto bytes = q.options().dtype(at::kByte);
-  Tensor y = out_bf16 ? at::empty({t, h * d}, x.options()) : at::empty({0}, x.options());
-  Tensor yp = out_planes ? at::empty({3, t, h * d}, bytes) : at::empty({0}, bytes);
+  Tensor y = out_bf16 ? new_tensor({t, h * d}, at::kBFloat16, x) : new_tensor({0}, at::kBFloat16, x);
+  Tensor yp = out_planes ? new_tensor({3, t, h * d}, at::kByte, x) : new_tensor({0}, at::kByte, x);
   if (t == 0) return {y, yp};
   const int64_t most = std::min(t, max_tokens.value_or(t));
   const size_t need = tybok_paged_attention_workspace_bytes(h, g, d, most);
-  const Tensor ws = at::empty({static_cast<int64_t>(need ? need : 1)}, bytes);
+  const Tensor ws = new_tensor({static_cast<int64_t>(need ? need : 1)}, at::kByte, x);
   const int64_t ks[3] = {kp.stride(0), kp.stride(1), kp.stride(2)}, vs[3] = {vp.stride(0), vp.stride(1), vp.stride(2)};
   check(tybok_paged_attention(ptr(x), x.stride(0), ptr(kp), ks, ptr(vp), vs, static_cast<const int*>(table.data_ptr()), table.stride(0),
                               static_cast<const int*>(cu.data_ptr()), static_cast<const int*>(lens.data_ptr()), out_bf16 ? ptr(y) : nullptr,

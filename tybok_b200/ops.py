@@ -902,7 +902,7 @@ def page_plan(key_lens, new_lens, block_table, free_pages, free_count, *, tokens
     if type(key_lens) is _Tensor:  # as w8a16_linear
         plan = _lib.native().page_plan(key_lens, new_lens, block_table, free_pages, free_count, tokens, page_size, finished, False)
         if plan is not None:
-            return PagePlan(*plan)
+            return tuple.__new__(PagePlan, plan)  # PagePlan(*plan), in half the time
     return PagePlan(*torch.ops.tybok_b200.page_plan(key_lens, new_lens, block_table, free_pages, free_count, tokens, page_size, finished))
 
 
