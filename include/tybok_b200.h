@@ -367,7 +367,8 @@ int tybok_head_norm_rope_store(const void* src, int64_t ld, const int* pos, cons
  * q[cu_tokens[b] .. cu_tokens[b+1]) (bf16 rows of H * D, row stride ldq) as the last of its key_lens[b] keys: query i of n sees
  * the keys j <= key_lens[b] - n + i (causal) or all of them; a query that sees none gives 0.  out bf16 [tokens][H * D] and /
  * or out_planes (e5m2 [3][tokens][H * D], scaled by 2^out_shift); rows of no request are 0.  What lies in pages behind a
- * request's last key is never read into a result.  max_tokens: the most tokens that a request brings, as far as the host
+ * request's last key is never read into a result.  A key that a query must not see takes part with weight 0, so values
+ * that are not finite among a request's own keys reach its other queries, as in a matrix product.  max_tokens: the most tokens that a request brings, as far as the host
  * knows (a choice between forms, not a limit).  Lengths and pages out of range are cut, or taken as zero keys and values, and
  * set the status word.  B <= 2048, D 128 or 256; any sign of scale. */
 int tybok_paged_attention(const void* q, int64_t ldq, const void* k_pages, const int64_t* k_strides, const void* v_pages,
