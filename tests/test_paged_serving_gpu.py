@@ -269,3 +269,19 @@ def test_requests_that_claim_the_same_tokens_are_reported(h, g, d):
     assert out.shape == q.shape
     y, _ = _check_attention((q, kp, vp, table, _i32([0, 40, 80, 120, 160, 200, 240]), _i32([60] * 6)), 0.1, False)  # and the next call is right
     assert y.shape == q.shape
+
+
+@pytest.mark.parametrize("most_keys", [64, 200])
+@pytest.mark.parametrize("tokens", [10, 3, 16])
+def test_many_short_tiles_in_a_row(tokens, most_keys):
+    """Hundreds of requests of one key block or a few at head_dim 256, so that a CTA's share runs through many tiles whose blocks fall to
+    one group of softmax warps alone, with warps that have no query rows; the same bits from run to run."""
+    from tybok_b200 import ops
+
+    rng = torch.Generator().manual_seed(tokens + most_keys)
+    lens = [int(x) for x in torch.randint(tokens, most_keys + 1, (700,), generator=rng)]
+    args = _attention_inputs(lens, [tokens] * 700, 8, 1, 256, 16, seed=14)
+    want, _ = _check_attention(args, 0.0625, False)
+    got = [ops.paged_attention(*args, scale=0.0625, causal=False)[0] for _ in range(100)]
+    ops.check_status()
+    assert all(torch.equal(want, y) for y in got)

@@ -770,8 +770,8 @@ struct __align__(16) PtBars {
   uint64_t p_full[2][4];         // the same, and 32 of the block's keys
   uint64_t done[2];              // pair: per tile, its last product has landed; wide: [block % 2], the block's product has
   uint64_t o_free;        // wide: the output of a tile has been read
-  uint64_t pub[2][4];     // wide: per group and warp: the reference maximum after this block; at the end of a tile, its sums
-  uint64_t fin[2][4];
+  uint64_t pub[2][4];     // wide: per group and warp: the reference maximum after this block
+  uint64_t fin[2][2][4];  // the same, per parity of the tile: its sums at the tile's end
   uint64_t mma_done;
   uint32_t tmem_base;
   volatile int abort;
@@ -1126,7 +1126,8 @@ __device__ __forceinline__ PaShare pt_begin(const PagedAttnParams& p, PtBars& ba
       for (int w = 0; w < 2; ++w) {
         mbar_init(&bars.p_full[w][i], 4);
         mbar_init(&bars.pub[w][i], 1);
-        mbar_init(&bars.fin[w][i], 1);
+        mbar_init(&bars.fin[0][w][i], 1);
+        mbar_init(&bars.fin[1][w][i], 1);
       }
     }
 #pragma unroll 1
@@ -1643,14 +1644,15 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         pt_hand_over<2>(live, bars.p_full[grp]);
       }
       if (!ok) break;
-      // both groups' sums, relative to the later reference
+      // Both groups' sums, relative to the later reference.  (With one barrier for all tiles a short next tile, whose blocks may all be the
+      // other group's, could be through before this one has asked.  The tile after that needs this group's sums of the next one.)
       bars.end_m[n & 1][grp][row] = m_own;
       bars.end_l[n & 1][grp][row] = l;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.fin[grp][q]);
+      if (lane == 0) mbar_arrive(&bars.fin[n & 1][grp][q]);
       any = reader.next(bars, next);
       if (!reader.ok || (any && !queries(n + 1))) break;  // the next scores may begin
-      if (!wait(&bars.fin[grp ^ 1][q], n & 1)) break;
+      if (!wait(&bars.fin[n & 1][grp ^ 1][q], (n >> 1) & 1)) break;
       const float m_other = bars.end_m[n & 1][grp ^ 1][row], m_end = fmaxf(m_own, m_other);
       l = l * pa_exp2(m_own - m_end) + bars.end_l[n & 1][grp ^ 1][row] * pa_exp2(m_other - m_end);
       if (!wait(&bars.done[(i - 1) & 1], ((i - 1) >> 1) & 1)) break;
