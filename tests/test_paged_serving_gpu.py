@@ -285,3 +285,19 @@ def test_many_short_tiles_in_a_row(tokens, most_keys):
     got = [ops.paged_attention(*args, scale=0.0625, causal=False)[0] for _ in range(100)]
     ops.check_status()
     assert all(torch.equal(want, y) for y in got)
+
+
+@pytest.mark.parametrize("requests", [3, 300])  # joined in clusters; a line of tiles
+@pytest.mark.parametrize("blocks", [3, 4, 5, 6, 7])
+def test_a_tile_ends_with_its_last_product(blocks, requests):
+    """Tiles of a few key blocks at head_dim 256 with scores so alike that no output row is ever rescaled: only the end of a tile waits for
+    a product.  The same bits from run to run."""
+    from tybok_b200 import ops
+
+    rng = torch.Generator().manual_seed(blocks)
+    lens = [64 * blocks - int(x) for x in torch.randint(0, 30, (requests,), generator=rng)]
+    args = _attention_inputs(lens, [12] * requests, 8, 1, 256, 16, seed=15)
+    want, _ = _check_attention(args, 0.01, False)
+    got = [ops.paged_attention(*args, scale=0.01, causal=False)[0] for _ in range(100)]
+    ops.check_status()
+    assert all(torch.equal(want, y) for y in got)

@@ -1614,7 +1614,12 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll 1
       for (int j = at.blk; j < at.end; ++j, ++i) {
         if ((i & 1) != static_cast<uint32_t>(grp)) continue;
-        ok = __all_sync(0xffffffffu, wait_or_abort(&bars.s_full[grp], (i >> 1) & 1, &bars.abort, p.wait_limit));
+        // The scores, and the product of this group's block before (half of the lanes each, in the time of one wait).  That product's next
+        // phase needs this block's weights, so nothing of it is missed here, and what this group has seen the other one knows by `pub`
+        // and `fin`: both can wait for either's last product below.  (The scores alone say that it has been done, not that its
+        // arrival is there: that is a commit of its own, and a wait for the phase after it would have passed at once.)
+        const bool product = (lane & 1) && i >= 2;
+        ok = __all_sync(0xffffffffu, wait_or_abort(product ? &bars.done[grp] : &bars.s_full[grp], product ? ((i >> 1) - 1) & 1 : (i >> 1) & 1, &bars.abort, p.wait_limit));
         if (!ok) break;
         uint32_t v[2][32];
         float m_blk = 0.f;
@@ -1632,8 +1637,8 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (lane == 0) mbar_arrive(&bars.pub[grp][q]);
         if (live) {
           if (__any_sync(0xffffffffu, grow) && j > at.blk) {
-            // The product before must have landed.  (These scores came after that of two blocks ago, so the barrier's phase before has
-            // passed, and its next waits for this block's weights.)
+            // The product before must have landed.  (The barrier's phase before has passed: the other group saw it before `pub`; its next waits
+            // for this block's weights.)
             if (!wait(&bars.done[(i - 1) & 1], ((i - 1) >> 1) & 1)) break;
             tc_fence_after();
             pt_rescale(t_o, 8, grow ? pa_exp2(m_ref - m_blk) : 1.0f);
