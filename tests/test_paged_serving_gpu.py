@@ -301,3 +301,31 @@ def test_a_tile_ends_with_its_last_product(blocks, requests):
     got = [ops.paged_attention(*args, scale=0.01, causal=False)[0] for _ in range(100)]
     ops.check_status()
     assert all(torch.equal(want, y) for y in got)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_a_plan_of_the_most_token_rows(in_place):
+    """2^31 - 1 token rows: the last stride of the threads over them passes 2^31."""
+    from tybok_b200 import ops
+
+    rows = 2**31 - 1
+    lens, table, free, count = _i32([40]), _i32([[3, 1, 0]]), _i32([2, 5, 4]), _i32([2])
+    plan = (ops.page_plan_ if in_place else ops.page_plan)(lens, _i32([7]), table, free, count, tokens=rows, page_size=16)
+    assert plan.missing.tolist() == [0] and plan.cu_tokens.tolist() == [0, 7] and plan.key_lens.tolist() == [47]
+    assert plan.block_table.tolist() == [[3, 1, 0]] and plan.free_pages.tolist() == [2, 5, 4] and plan.free_count.tolist() == [2]
+    assert plan.pos[:8].tolist() == [*range(40, 47), 0] and plan.slots[:8].tolist() == [*range(8, 15), -1]
+    for t, behind in ((plan.pos, 0), (plan.slots, -1)):
+        assert t.numel() == rows and all(bool((part == behind).all()) for part in t[7:].split(1 << 28))
+
+
+def test_a_request_that_grows_to_the_most_keys():
+    """Lengths, positions and token numbers next to 2^31, in one request and behind others."""
+    from tybok_b200 import ops
+
+    page, top = 1 << 20, 2**31 - 1
+    table = torch.arange(2 * 2048, dtype=torch.int32, device="cuda").view(2, 2048) % 2000
+    plan = ops.page_plan(_i32([0, top - 3000]), _i32([5000, 3000]), table, _i32([7] * 2000), _i32([9]), tokens=8000, page_size=page)
+    assert plan.missing.tolist() == [0] and plan.key_lens.tolist() == [5000, top] and plan.cu_tokens.tolist() == [0, 5000, 8000]
+    assert plan.pos[5000:].tolist() == list(range(top - 3000, top))
+    last = int(table[1, 2047])
+    assert plan.slots[5000:].tolist() == [last * page + p % page for p in range(top - 3000, top)]

@@ -148,11 +148,11 @@ __global__ void __launch_bounds__(1024) page_plan_kernel(const PlanParams p) {
   } else {
     for (int i = g0; i < p.P; i += gn) p.stack_out[i] = i >= count && i < count + nback ? back_page(i - count) : p.stack[i];
     for (int b = g0 >> 5; b < p.B; b += gn >> 5) {  // a warp per row; the entries that are new come below
-      const int keep = ok ? plan_pages(base[b], p.page_shift) : p.W, to = keep + (ok ? more[b + 1] - more[b] : 0);
+      const unsigned keep = ok ? plan_pages(base[b], p.page_shift) : p.W, to = keep + (ok ? more[b + 1] - more[b] : 0), width = p.W;
       const int* src = p.table + static_cast<long long>(b) * p.W;
       int* dst = p.table_out + static_cast<long long>(b) * p.W;
 #pragma unroll 4
-      for (int j = lane; j < p.W; j += 32)
+      for (unsigned j = lane; j < width; j += 32)
         if (j < keep || j >= to) dst[j] = src[j];
     }
   }
@@ -169,11 +169,12 @@ __global__ void __launch_bounds__(1024) page_plan_kernel(const PlanParams p) {
     p.table_out[static_cast<long long>(b) * p.W + plan_pages(base[b], p.page_shift) + x - more[b]] = taken(x);
   }
   const int page = 1 << p.page_shift, real = ok ? cu[p.B] : 0;
-  for (int t = g2; t < p.T; t += gn) {
+  for (unsigned i = g2; i < static_cast<unsigned>(p.T); i += gn) {  // (in 31 bits the last stride could go round and below zero)
+    const int t = static_cast<int>(i);
     int at = 0, slot = -1;
     if (t < real) {
       const int b = plan_find(cu, p.B, t);
-      at = base[b] + t - cu[b];
+      at = base[b] + (t - cu[b]);
       const int j = at >> p.page_shift, keep = plan_pages(base[b], p.page_shift);
       const int number = j < keep ? p.table[static_cast<long long>(b) * p.W + j] : taken(more[b] + j - keep);
       slot = number * page + (at & (page - 1));
@@ -183,7 +184,7 @@ __global__ void __launch_bounds__(1024) page_plan_kernel(const PlanParams p) {
   }
   for (int b = g0; b <= p.B; b += gn) p.cu[b] = ok ? cu[b] : 0;
   for (int b = g0; b < p.B; b += gn) {
-    if (ok) p.lens_out[b] = base[b] + cu[b + 1] - cu[b];
+    if (ok) p.lens_out[b] = base[b] + (cu[b + 1] - cu[b]);
     else if (!p.in_place) p.lens_out[b] = p.lens[b];
   }
   if (g0 == 0) {
