@@ -329,3 +329,23 @@ def test_a_request_that_grows_to_the_most_keys():
     assert plan.pos[5000:].tolist() == list(range(top - 3000, top))
     last = int(table[1, 2047])
     assert plan.slots[5000:].tolist() == [last * page + p % page for p in range(top - 3000, top)]
+
+
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("new", [1, 100])
+@pytest.mark.parametrize("causal", [True, False])
+def test_scores_near_the_lowest_value(d, new, causal):
+    """Finite scores far below -1e30: equal ones average their values, and among unequal ones the highest alone counts.  They are single
+    products of powers of two, so exact, and differ by nothing or by more than any exponential can tell: the bound of
+    ``_check_attention`` holds as it is."""
+    q, kp, vp, table, cu, lens = _attention_inputs([900], [new], 2, 1, d, 16, seed=16)
+    q.zero_()
+    q.view(new, 2, d)[:, :, 0] = 2.0**60
+    at = torch.arange(900, device="cuda")
+    for some in (2.0**60, 2.0**62):  # the scores of two keys of three; the others' are -2^118, -3e35
+        kp[table[0, at // 16].long(), 0, at % 16] = 0
+        kp[table[0, at // 16].long(), 0, at % 16, 0] = torch.where(at % 3 == 0, -(2.0**60), -some).to(torch.bfloat16)
+        _check_attention((q, kp, vp, table, cu, lens), 0.25, causal)
+    for clip in (130, 900):  # keys before these have the lowest of all, and the first rows see no others
+        kp[table[0, at // 16].long(), 0, at % 16, 0] = torch.where(at < clip, -(2.0**66), 0.0).to(torch.bfloat16)
+        _check_attention((q, kp, vp, table, cu, lens), 0.25, causal)

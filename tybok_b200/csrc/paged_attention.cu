@@ -721,6 +721,9 @@ constexpr int PT_REGS_CONTROL = 72, PT_REGS_SOFTMAX = 216;  // launched with 168
 constexpr int PT_SMEM = 196608 + 1024;  // queries, two key and two value blocks
 constexpr float PT_RESCALE = 8.0f;
 #define PA_MASKED 0xff800000u  // -infinity
+// Where a row's reference starts, and its least value: finite, so that a masked score's distance from it is -infinity and not NaN, and
+// below every finite score.
+constexpr float PT_LOWEST = -3.402823466e38f;
 
 __host__ __device__ constexpr int pt_rows(int d) { return d == 128 ? 256 : 128; }  // of a work item
 __host__ __device__ constexpr int pt_bk(int d) { return d == 128 ? 128 : 64; }     // keys of a block (32 KB)
@@ -1166,7 +1169,7 @@ __device__ __forceinline__ PaShare pt_begin(const PagedAttnParams& p, PtBars& ba
 template <int N>
 __device__ __forceinline__ float pt_scores(uint32_t t_s, uint32_t (&v)[N][32], int seen, float scale) {
   tc_fence_after();
-  float mx[4] = {-1e30f, -1e30f, -1e30f, -1e30f};
+  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
   tmem_ld32(t_s, v[0]);
 #pragma unroll
   for (int w = 0; w < N; ++w) {  // 32 scores' maximum under the load of the next ones
@@ -1175,7 +1178,7 @@ __device__ __forceinline__ float pt_scores(uint32_t t_s, uint32_t (&v)[N][32], i
     if (w + 1 < N) tmem_ld32(t_s + (w + 1) * 32, v[w + 1 < N ? w + 1 : 0]);
     pt_row_max<4>(v[w], seen - 32 * w, mx);
   }
-  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+  return fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale, PT_LOWEST);
 }
 // ... and the weights relative to m over them, handed over 32 keys at a time (the last ones by the caller); returns their sum.
 template <int N>
@@ -1393,7 +1396,7 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       if (nvalid <= 0) continue;
       const bool live = q * 32 < nvalid, mine = row < nvalid;
       const int limit = at.seen + ahead * at.step;  // keys this row sees
-      float m_ref = -1e30f, l = 0.f;
+      float m_ref = PT_LOWEST, l = 0.f;
 #pragma unroll 1
       for (int j = at.blk; j < at.end; ++j, ++i) {
         ok = __all_sync(0xffffffffu, wait_or_abort(&bars.s_full[t], i & 1, &bars.abort, p.wait_limit));
@@ -1610,7 +1613,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     for (uint32_t n = 0; any; ++n) {
       const bool live = q * 32 < at.rows, mine = row < at.rows;
       const int limit = at.seen + ahead * at.step;
-      float m_own = -1e30f, l = 0.f;  // the reference that l is relative to
+      float m_own = PT_LOWEST, l = 0.f;  // the reference that l is relative to
 #pragma unroll 1
       for (int j = at.blk; j < at.end; ++j, ++i) {
         if ((i & 1) != static_cast<uint32_t>(grp)) continue;
@@ -1625,7 +1628,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         float m_blk = 0.f;
         if (live) m_blk = pt_scores<2>(t_s, v, limit - j * BK, p.abs_scale_log2e);
         // the reference after the block before, which the other group has
-        float m_ref = -1e30f;
+        float m_ref = PT_LOWEST;
         if (j > at.blk) {
           if (!wait(&bars.pub[grp ^ 1][q], ((i - 1) >> 1) & 1)) break;
           m_ref = bars.m_ref[grp ^ 1][row];
