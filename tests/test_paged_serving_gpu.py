@@ -349,3 +349,17 @@ def test_scores_near_the_lowest_value(d, new, causal):
     for clip in (130, 900):  # keys before these have the lowest of all, and the first rows see no others
         kp[table[0, at // 16].long(), 0, at % 16, 0] = torch.where(at < clip, -(2.0**66), 0.0).to(torch.bfloat16)
         _check_attention((q, kp, vp, table, cu, lens), 0.25, causal)
+
+
+def test_results_of_the_registered_plans_share_no_memory():
+    """As their schemas say; the direct call's are pieces of one allocation, apart from the state in place."""
+    from tybok_b200 import ops
+
+    state = lambda: (_i32([16, 4]), _i32([1, 2]), torch.zeros(2, 5000, dtype=torch.int32, device="cuda"), _i32([2, 3, 0]), _i32([2]))  # noqa: E731
+    where = lambda t: t.untyped_storage().data_ptr()  # noqa: E731
+    plan, own = ops.page_plan(*state(), tokens=3, page_size=16), ops.page_plan_(*state(), tokens=3, page_size=16)
+    for t in (own.cu_tokens, own.pos, own.slots, own.missing):
+        assert where(t) != where(own.block_table) and t.untyped_storage().nbytes() < 4096
+    for out in (torch.ops.tybok_b200.page_plan(*state(), 3, 16, None), torch.ops.tybok_b200.page_plan_(*state(), 3, 16, None)):
+        assert len({where(t) for t in out}) == len(out)
+        assert all(torch.equal(a, b) for a, b in zip(out, plan if len(out) == 8 else plan[4:]))

@@ -898,7 +898,9 @@ _L.impl("paged_attention", _paged_attention_cuda, "CUDA")
 def page_plan(key_lens, new_lens, block_table, free_pages, free_count, *, tokens, page_size, finished=None) -> PagePlan:
     """The pages of a step, planned on the GPU from the requests' lengths: requests that are ``finished`` return theirs and start
     anew at length 0, then every request gets the pages that its ``new_lens`` tokens need.  ``tokens`` is the number of token
-    rows of the step (padding behind the last token included).  The given state is left as it is; see ``tybok_page_plan``."""
+    rows of the step (padding behind the last token included).  The given state is left as it is; see ``tybok_page_plan``.
+    The result's tensors are pieces of one allocation: whoever keeps one of them keeps that much memory (``.clone()`` does not; nor
+    does ``page_plan_``, whose result holds the step's own four alone)."""
     if type(key_lens) is _Tensor:  # as w8a16_linear
         plan = _lib.native().page_plan(key_lens, new_lens, block_table, free_pages, free_count, tokens, page_size, finished, False)
         if plan is not None:
