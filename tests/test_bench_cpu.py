@@ -64,3 +64,9 @@ def test_traffic_record_is_reported_only_for_the_sources_it_was_captured_on(monk
     assert traffic is None and note.startswith("stale")
     monkeypatch.setattr(bench, "TRAFFIC_FILE", str(tmp_path / "missing.json"))
     assert bench._traffic()[0] is None
+
+
+def test_the_committed_traffic_record_is_of_the_committed_sources():
+    """A change of the sources that it names comes with a new capture: otherwise the benchmark's line loses the figure."""
+    traffic, note = bench._traffic()
+    assert traffic == json.load(open(bench.TRAFFIC_FILE))["dram_bytes_per_launch"], note

@@ -750,6 +750,15 @@ __device__ __forceinline__ uint64_t pt_add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// 4-D tiled load (crd0 innermost).
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, uint64_t* bar, int crd0, int crd1, int crd2, int crd3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(crd0), "r"(crd1), "r"(crd2), "r"(crd3)
+      : "memory");
+}
+
 // What the CTA does with (a piece of) a tile.
 struct __align__(16) PtPiece {
   int rows;         // query rows of the tile; 0 = the share is through
