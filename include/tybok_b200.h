@@ -356,7 +356,8 @@ int tybok_page_plan(const int* key_lens, const int* new_lens, const void* finish
  * first `rot` channels rotated by the angles of the row's position (cos / sin fp32 [max_pos][rot / 2]; pairs i and
  * i + rot / 2, or 2i and 2i + 1 with `paired`), one rounding to bf16.  q goes to q_out [tokens][H * D], k and the untouched
  * v to slots[row] of their pools; rows with a negative slot store neither.  A position outside the tables or a slot outside the
- * pool sets the status word; such a row is not stored (and its q is 0 where the position is out).  Slots must differ. */
+ * pool sets the status word; such a row is not stored (and its q is 0 where the position is out).  Slots must differ, and the pools'
+ * rows must not overlap (a pool whose strides make them do so is refused, and one pool for both).  rot is a multiple of 16. */
 int tybok_head_norm_rope_store(const void* src, int64_t ld, const int* pos, const int* slots, const float* cos_table,
                                const float* sin_table, int max_pos, int rot, int paired, const float* norm_q, const float* norm_k,
                                float eps, void* q_out, void* k_pages, const int64_t* k_strides, void* v_pages,

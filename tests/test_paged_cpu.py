@@ -151,3 +151,37 @@ def test_workspace_is_bounded():
     for h, g, d, n in ((8, 1, 256, 1), (8, 1, 256, 50), (32, 8, 128, 4096), (1, 1, 128, 1 << 20)):
         assert 0 < lib.tybok_paged_attention_workspace_bytes(h, g, d, n) <= 100 << 20
     assert lib.tybok_paged_attention_workspace_bytes(8, 1, 64, 1) == 0
+
+
+SAME = _bf(P, G, PAGE, D)
+
+
+@pytest.mark.parametrize("over", [
+    dict(k_pages=SAME, v_pages=SAME),
+    dict(k_pages=_bf(P * G * PAGE * D).as_strided((P, G, PAGE, D), (G * PAGE * D, PAGE * D, D // 2, 1))),  # rows half on one another
+    dict(v_pages=_bf(P * G * PAGE * D).as_strided((P, G, PAGE, D), (PAGE * D, PAGE * D, D, 1))),  # heads in the next page
+    dict(v_pages=_bf(P * G * PAGE * D).as_strided((P, G, PAGE, D), (8, PAGE * D, D, 1))),
+])
+def test_store_refuses_rows_on_top_of_one_another(over):
+    with pytest.raises(ValueError, match="overlap"):
+        _store(**over)
+
+
+@pytest.mark.parametrize("shape,strides", [
+    ((P, G, PAGE, D), (D, P * D, P * G * D, 1)), ((P, 1, PAGE, D), (PAGE * D, 8, D, 1)), ((1, G, PAGE, D), (8, D, G * D, 1)),
+    ((P, G, PAGE, D), (2 * G * PAGE * (D + 8), PAGE * (D + 8), D + 8, 1)),
+])
+def test_store_takes_any_order_of_rows_that_lie_apart(shape, strides):
+    pool = lambda: _bf(4 * P * G * PAGE * D).as_strided(shape, strides)  # noqa: E731
+    heads = H + 2 * G - 2 * shape[1]
+    with pytest.raises(NotImplementedError, match="no CPU implementation|'CPU' backend"):
+        _store(k_pages=pool(), v_pages=pool(), heads=heads)
+
+
+@pytest.mark.parametrize("over", [
+    dict(v=ctypes.c_void_p(16)), dict(ks=(ctypes.c_int64 * 3)(G * PAGE * D, PAGE * D, D - 8)), dict(vs=(ctypes.c_int64 * 3)(PAGE * D, PAGE * D, D)),
+    dict(ks=(ctypes.c_int64 * 3)(1 << 62, 1 << 62, D)),
+])
+def test_c_store_refuses_rows_on_top_of_one_another(over):
+    rc, message = _c("tybok_head_norm_rope_store", **{"v": ctypes.c_void_p(32), **over})
+    assert rc != 0 and "overlap" in message

@@ -1,6 +1,8 @@
 // The paged cache: page plan, head norms with rotation and store, attention over pages.
 #include <ATen/cuda/EmptyTensor.h>
 
+#include <algorithm>
+
 #include "native.h"
 
 namespace tbn {
@@ -89,12 +91,26 @@ static void need_pool(const Tensor& t, const char* what, const char* name) {
   if (t.size(0) > 0x7fffffff || t.size(2) > 0x7fffffff) value_error(who + ": pages and their size must be 31-bit numbers");
 }
 
+// Whether a pool's rows share no element: each stride, from the smallest up, passes over all that lies inside it.
+static bool rows_apart(const Tensor& t) {
+  int order[3] = {0, 1, 2};
+  std::sort(order, order + 3, [&](int a, int b) { return t.stride(a) < t.stride(b); });
+  int64_t inside = t.size(3);
+  for (const int i : order) {
+    if (t.size(i) == 1) continue;
+    if (t.stride(i) < inside) return false;
+    inside += t.stride(i) * (t.size(i) - 1);
+  }
+  return true;
+}
+
 static Tensor head_norm_rope_store(const Tensor& qkv, const Tensor& pos, const Tensor& slots, const Tensor& cos, const Tensor& sin, const Tensor& kp,
                                    const Tensor& vp, int64_t heads, const OptTensor& norm_q, const OptTensor& norm_k, double eps, bool paired) {
   const char* what = "head_norm_rope_store";
   need_pool(kp, what, "k_pages");
   need_pool(vp, what, "v_pages");
   if (kp.sizes() != vp.sizes()) value_error("head_norm_rope_store: key and value pages differ in shape");
+  if (!rows_apart(kp) || !rows_apart(vp) || kp.data_ptr() == vp.data_ptr()) value_error("head_norm_rope_store: rows of the pools must not overlap");
   const int64_t g = kp.size(1), page = kp.size(2), d = kp.size(3);
   if (!is_bf16(qkv) || qkv.dim() != 2) type_error("head_norm_rope_store: qkv must be bf16 [tokens, (H + 2G) * D]");
   if (heads < 1 || qkv.size(1) != (heads + 2 * g) * d) value_error("head_norm_rope_store: the rows of qkv must hold H + 2G heads");

@@ -408,6 +408,19 @@ __global__ void __launch_bounds__(HN_THREADS, 8) head_norm_rope_store_kernel(con
   }
 }
 
+// Whether rows of `d` elements at these strides share none: each stride, from the smallest up, passes over all that lies inside it.
+static bool rows_apart(const int64_t* strides, const int (&extents)[3], int d) {
+  int order[3] = {0, 1, 2};
+  std::sort(order, order + 3, [&](int a, int b) { return strides[a] < strides[b]; });
+  __int128 inside = d;
+  for (const int i : order) {
+    if (extents[i] <= 1) continue;
+    if (strides[i] < inside) return false;
+    inside += static_cast<__int128>(strides[i]) * (extents[i] - 1);
+  }
+  return true;
+}
+
 static int page_shift_of(int page) {
   if (page < 16 || (page & (page - 1))) return -1;
   int s = 4;
@@ -502,6 +515,8 @@ int tybok_head_norm_rope_store(const void* src, int64_t ld, const int* pos, cons
   for (int i = 0; i < 3; ++i) strides |= k_strides[i] | v_strides[i];
   if ((bits & 15) || (strides & 7))
     return host::fail(TYBOK_ERR_ARG, "head_norm_rope_store: tensors must be 16-byte aligned, strides multiples of 8 elements");
+  if (!rows_apart(k_strides, extents, D) || !rows_apart(v_strides, extents, D) || k_pages == v_pages)
+    return host::fail(TYBOK_ERR_ARG, "head_norm_rope_store: rows of the pools must not overlap");
   if (int rc = host::require_sm100()) return rc;
   HeadNormParams p{};
   p.src = static_cast<const __nv_bfloat16*>(src); p.ld = ld; p.pos = pos; p.slots = slots; p.cos = cos_table; p.sin = sin_table;
