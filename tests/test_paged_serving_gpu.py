@@ -363,3 +363,31 @@ def test_results_of_the_registered_plans_share_no_memory():
     for out in (torch.ops.tybok_b200.page_plan(*state(), 3, 16, None), torch.ops.tybok_b200.page_plan_(*state(), 3, 16, None)):
         assert len({where(t) for t in out}) == len(out)
         assert all(torch.equal(a, b) for a, b in zip(out, plan if len(out) == 8 else plan[4:]))
+
+
+@pytest.mark.parametrize("h,g,d,most", [(8, 1, 256, 240), (8, 2, 128, 240), (1, 1, 128, 1), (8, 1, 256, 1)])
+@pytest.mark.parametrize("cu,lens", [([0, 240, 0, 240, 0, 240, 0], [60] * 6), ([0, -5, 300, 240, 1 << 30, -(1 << 31), 7], [60, 1 << 30, -1, 0, 500, 3]),
+                                     ([230, 240, 250, 260, 0, 10, 500], [400] * 6)])
+def test_bounds_out_of_range_touch_no_byte_around_the_outputs(h, g, d, most, cu, lens):
+    """Through the C entry point, with outputs, planes and workspace inside larger tensors of a pattern."""
+    import ctypes
+
+    from tybok_b200 import _lib, ops
+
+    q, kp, vp, table, _, _ = _attention_inputs([60] * 6, [40] * 6, h, g, d, 16, seed=12)
+    lib, n, edge = _lib.load(), q.numel(), 1 << 20
+    need = lib.tybok_paged_attention_workspace_bytes(h, g, d, most)
+    whole = {"out": torch.full((2 * n + 2 * edge,), 0x5A, dtype=torch.uint8, device="cuda"),
+             "planes": torch.full((3 * n + 2 * edge,), 0x5A, dtype=torch.uint8, device="cuda"),
+             "ws": torch.full((need + 2 * edge,), 0x5A, dtype=torch.uint8, device="cuda")}
+    strides = lambda t: (ctypes.c_int64 * 3)(*t.stride()[:3])  # noqa: E731
+    word = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cu_t, lens_t = _i32(cu), _i32(lens)
+    at = {name: t.data_ptr() + edge for name, t in whole.items()}
+    rc = lib.tybok_paged_attention(q.data_ptr(), q.stride(0), kp.data_ptr(), strides(kp), vp.data_ptr(), strides(vp), table.data_ptr(), table.stride(0),
+                                   cu_t.data_ptr(), lens_t.data_ptr(), at["out"], at["planes"], 3, q.shape[0], 6, h, g, d, kp.shape[0], 16, table.shape[1],
+                                   most, 0, 0.08, at["ws"], need, word.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, lib.tybok_last_error()
+    assert word.item() == ops.DEV_BAD_INDEX
+    for name, t in whole.items():
+        assert bool((t[:edge] == 0x5A).all()) and bool((t[-edge:] == 0x5A).all()), name

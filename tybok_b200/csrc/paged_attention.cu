@@ -75,7 +75,7 @@ __device__ __forceinline__ PaRequest pa_request(const PagedAttnParams& p, int b)
   PaRequest r;
   const int lo = p.cu[b], hi = p.cu[b + 1];
   r.start = max(0, min(lo, p.T));
-  r.n = max(0, min(hi, p.T) - r.start);
+  r.n = max(r.start, min(hi, p.T)) - r.start;  // (cut before the difference, which could go round for a bound near -2^31)
   r.len = static_cast<int>(min(static_cast<long long>(max(0, p.lens[b])), static_cast<long long>(p.W) << p.page_shift));
   return r;
 }
