@@ -481,19 +481,19 @@ __global__ void __launch_bounds__(PR_THREADS, pr_ctas(D)) paged_rows_kernel(cons
     };
     uint32_t qf[KS][4];
     int limit[2];
-        // this thread's two rows of the tile: queries as operand fragments, keys they see
+    // this thread's two rows of the tile: queries as operand fragments, keys they see
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = at.tile * PR_ROWS + h * 8 + (lane >> 2), token = pa_token(p, row);
-          const bool live = row < rows;
-          limit[h] = !live ? 0 : p.causal ? max(0, at.r.len - at.r.n + token + 1) : at.r.len;
-          const __nv_bfloat16* src = p.q + (at.r.start + token) * p.ldq + static_cast<long long>(at.g * p.ratio + row - token * p.ratio) * D + (lane & 3) * 2;
+    for (int h = 0; h < 2; ++h) {
+      const int row = at.tile * PR_ROWS + h * 8 + (lane >> 2), token = pa_token(p, row);
+      const bool live = row < rows;
+      limit[h] = !live ? 0 : p.causal ? max(0, at.r.len - at.r.n + token + 1) : at.r.len;
+      const __nv_bfloat16* src = p.q + (at.r.start + token) * p.ldq + static_cast<long long>(at.g * p.ratio + row - token * p.ratio) * D + (lane & 3) * 2;
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            qf[ks][h] = live ? *reinterpret_cast<const uint32_t*>(src + ks * 16) : 0u;
-            qf[ks][h + 2] = live ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8) : 0u;
-          }
-        }
+      for (int ks = 0; ks < KS; ++ks) {
+        qf[ks][h] = live ? *reinterpret_cast<const uint32_t*>(src + ks * 16) : 0u;
+        qf[ks][h + 2] = live ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8) : 0u;
+      }
+    }
     float o[D / 8][4];
 #pragma unroll
     for (int i = 0; i < D / 8; ++i)
@@ -962,15 +962,15 @@ __device__ __forceinline__ void pt_lead(const PagedAttnParams& p, PaPlace at, co
   if (lane == 0 && !p.cluster) reinterpret_cast<PaHeader*>(p.ws)[blockIdx.x] = header;
 }
 
-// Keys (values) of the share: one block after the other into a ring of two.  A block's boxes: lane = piece of the block * chunks + chunk of
-// 64 channels.  A warp may look after both rings.  Stays until its last copies have landed.
+// Keys or values of the share: one block after the other into a ring of two.  A block's boxes: lane = piece of the block * chunks + chunk of
+// 64 channels.  Stays until its last copies have landed.
 struct PtRing {
   const CUtensorMap* map;
   uint8_t* at;
   uint64_t *full, *empty;
 };
-template <int D, int N>
-__device__ __forceinline__ void pt_stream(const PagedAttnParams& p, const PtRing (&rings)[N], PtBars& bars) {
+template <int D>
+__device__ __forceinline__ void pt_stream(const PagedAttnParams& p, const PtRing& ring, PtBars& bars) {
   constexpr int BK = pt_bk(D), NCH = D / 64, BYTES = BK * D * 2;
   const int lane = threadIdx.x & 31, rows = min(BK, 1 << p.page_shift), chunk = lane % NCH, row = lane / NCH * rows;
   // This lane's page of block j: -1 where nothing is to be copied, P (out of the map's bounds: zeros) for a bad number.
@@ -984,7 +984,7 @@ __device__ __forceinline__ void pt_stream(const PagedAttnParams& p, const PtRing
     }
     return n;
   };
-  uint32_t blocks[N] = {}, i = 0;  // blocks requested per ring; blocks begun
+  uint32_t blocks = 0, i = 0;  // blocks requested; blocks begun
   bool ok = true;
   PtReader reader;
   PtPiece at{};
@@ -995,21 +995,16 @@ __device__ __forceinline__ void pt_stream(const PagedAttnParams& p, const PtRing
       const int now = page, s = i & 1, off = (j * BK + row) & ((1 << p.page_shift) - 1);
       if (j + 1 < at.end) page = page_of(at, j + 1);
       const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, now >= 0)) * rows * 128, par = ((i >> 1) & 1) ^ 1;
-#pragma unroll
-      for (int r = 0; r < N; ++r) {
-        if (i >= 2) ok = ok && __all_sync(0xffffffffu, wait_or_abort(&rings[r].empty[s], par, &bars.abort));
-        if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(&rings[r].full[s], bytes);
-        __syncwarp();
-        if (now >= 0) tma_load_4d(rings[r].at + s * BYTES + chunk * (BK * 128) + row * 128, rings[r].map, &rings[r].full[s], chunk * 64, off, at.g, now);
-        blocks[r] = i + 1;
-      }
+      if (i >= 2) ok = __all_sync(0xffffffffu, wait_or_abort(&ring.empty[s], par, &bars.abort));
+      if (!ok) break;
+      if (lane == 0) mbar_arrive_expect_tx(&ring.full[s], bytes);
+      __syncwarp();
+      if (now >= 0) tma_load_4d(ring.at + s * BYTES + chunk * (BK * 128) + row * 128, ring.map, &ring.full[s], chunk * 64, off, at.g, now);
+      blocks = i + 1;
     }
   }
   __syncwarp();
-#pragma unroll
-  for (int r = 0; r < N; ++r)
-    for (uint32_t k = blocks[r] < 2 ? 0 : blocks[r] - 2; k < blocks[r]; ++k) mbar_wait(&rings[r].full[k & 1], (k >> 1) & 1);
+  for (uint32_t k = blocks < 2 ? 0 : blocks - 2; k < blocks; ++k) mbar_wait(&ring.full[k & 1], (k >> 1) & 1);
 }
 
 // Zero the values of block j that lie behind the request's last key.  By a whole warp, after the block has landed.
@@ -1308,8 +1303,7 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       pt_lead<D>(p, first, share, &tm_q, sq, bars);
     } else if (warp != 1) {
       const bool k = warp == 0;
-      const PtRing rings[1] = {{k ? &tm_k : &tm_v, k ? sk : sv, k ? bars.k_full : bars.v_full, k ? bars.k_empty : bars.v_empty}};
-      pt_stream<D, 1>(p, rings, bars);
+      pt_stream<D>(p, {k ? &tm_k : &tm_v, k ? sk : sv, k ? bars.k_full : bars.v_full, k ? bars.k_empty : bars.v_empty}, bars);
     } else {
       const uint32_t leader = elect_one();
       const uint32_t idesc_s = idesc_bf16_f32(128, BK) | p.negate_q, idesc_o = idesc_bf16_f32(128, D) | (1u << 16);
@@ -1495,8 +1489,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     } else if (warp != 1) {
       const bool k = warp == 0;
       // a key block's place is free when its scores are there, a value block's when its product is: no barriers of their own
-      const PtRing rings[1] = {{k ? &tm_k : &tm_v, k ? sk : sv, k ? bars.k_full : bars.v_full, k ? bars.s_full : bars.done}};
-      pt_stream<D, 1>(p, rings, bars);
+      pt_stream<D>(p, {k ? &tm_k : &tm_v, k ? sk : sv, k ? bars.k_full : bars.v_full, k ? bars.s_full : bars.done}, bars);
     } else {
       const uint32_t leader = elect_one();
       const uint32_t idesc_s = idesc_bf16_f32(128, BK) | p.negate_q, idesc_o = idesc_bf16_f32(128, D) | (1u << 16);
@@ -1765,7 +1758,7 @@ __global__ void __launch_bounds__(128) paged_join_tile_kernel(const PagedAttnPar
 }
 
 // The same for the sixteen-row form; a warp per row.
-template <int ROWS, int D>
+template <int D>
 __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnParams p, int ctas) {
   if (p.pdl) {
     pdl_launch_dependents();
@@ -1773,6 +1766,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnParams p
   }
   const PaHeader h = reinterpret_cast<const PaHeader*>(p.ws)[blockIdx.x];
   if (h.parts == 0) return;
+  constexpr int ROWS = PR_ROWS;
   const uint8_t* parts = p.ws + pa_header_bytes(ctas);
   auto part = [&](int i) {  // the i-th part of the tile
     return reinterpret_cast<const float*>(parts + (2ll * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * pa_part_bytes<ROWS, D>());
@@ -1992,7 +1986,7 @@ int tybok_paged_attention(const void* q, int64_t ldq, const void* k_pages, const
   cfg.blockDim = dim3(128);
   cfg.dynamicSmemBytes = 0;
   PaJoinKernel* join = tiles ? (D == 256 ? paged_join_tile_kernel<256> : paged_join_tile_kernel<128>)
-                             : (D == 256 ? paged_join_kernel<PR_ROWS, 256> : paged_join_kernel<PR_ROWS, 128>);
+                             : (D == 256 ? paged_join_kernel<256> : paged_join_kernel<128>);
   if (cudaLaunchKernelEx(&cfg, join, p, ctas) != cudaSuccess) return host::fail_cuda("launch paged_join_kernel");
   host::count_launch();
   return TYBOK_OK;
