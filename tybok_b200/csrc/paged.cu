@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(1024) page_plan_kernel(const PlanParams p) {
     if (p.in_place) return __ldcg(p.stack_out + i);
     return i < count ? p.stack[i] : back_page(i - count);
   };
-  // The rest begins with other CTAs than the copies: each part is a chain of its own (48 requests 3.7 us against 5.1, 2048 requests 6.0 against 8.8).
+  // The rest begins with other CTAs than the copies: each part is a chain of its own (48 requests 3.8 us against 5.1, 2048 requests 6.0 against 8.8).
   const int half = gridDim.x >> 1, g1 = (blockIdx.x < half ? blockIdx.x + gridDim.x - half : blockIdx.x - half) * n + tid;
   const int g2 = (gridDim.x - 1 - blockIdx.x) * n + tid;
   for (int x = g1; x < nmore; x += gn) {

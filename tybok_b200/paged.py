@@ -4,10 +4,14 @@ The caches of ``PI05Model`` are ``[B, G, keys, D]``: every request takes the roo
 pages for the tokens that it has, whatever the others hold; which page serves whom is planned on the GPU
 (``ops.page_plan_``), so a step of a server is three kinds of launches and can be captured into a graph::
 
-    cache = PagedCache(layers=18, requests=16, pages=4096, page_size=16, kv_heads=1, head_dim=256)
-    plan = cache.step(new_lens, tokens=rows, finished=left)      # once per step
-    for i, layer in enumerate(decoder):
-        out, _ = cache.attend(i, layer.qkv(x), cos, sin, heads=8)  # norms, rotation, store, attention
+    cache = PagedCache(layers=18, requests=16, pages=4096, page_size=16, kv_heads=1, head_dim=256, width=128)
+    plan = cache.step(new_lens, tokens=16, finished=left)        # once per step; here of single tokens
+    for i, layer in enumerate(decoder):                          # norms, rotation, store, attention
+        out, _ = cache.attend(i, layer.qkv(x), cos, sin, heads=8, max_tokens=1)
+
+``width`` (the most pages of one request) and ``max_tokens`` (the most tokens that one request brings to the step) choose between forms of
+the attention and change no more than rounding.  Without them the host has to allow for requests as long as the pool and
+for a step that is all one request's: single tokens then take the kernels of whole prompts.
 
 The counterpart of the key/value caches that the reference's decoder keeps per request (tybok/policies/pi05/models/gemma.py:61-125).
 """
@@ -63,7 +67,8 @@ class PagedCache:
                out_shift: int = DEFAULT_SHIFT) -> tuple[torch.Tensor, torch.Tensor]:
         """One layer of the planned step: the projection rows ``qkv`` ``[tokens, (heads + 2 * kv_heads) * head_dim]`` are normed, rotated and
         stored, and every request's new tokens attend to all its keys.  Returns ``(out_bf16, out_planes)`` as ``ops.paged_attention``
-        does; ``scale`` is ``head_dim ** -0.5`` unless given."""
+        does; ``scale`` is ``head_dim ** -0.5`` unless given.  ``max_tokens``: as there, the step's token rows unless given, so a step of single
+        tokens is quickest with ``max_tokens=1``."""
         if self.plan is None:
             raise RuntimeError("attend() before the first step()")
         if not 0 <= layer < self.k_pages.shape[0]:
